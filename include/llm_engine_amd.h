@@ -102,6 +102,28 @@ int le_rope_kv_cache_write(const void* qkv, le_dtype act_dtype, int64_t qkv_row_
                            le_dtype cache_dtype, int64_t num_slots, hipStream_t stream);
 
 /* ------------------------------------------------------------------------
+ * (2) The same for models that normalise each query and key head before the
+ * rotation (no counterpart in the reference):
+ *     x += bias (if not NULL, fp32)
+ *     every q and k head: x = x / sqrt(mean(x^2) + eps) * w, w = q_norm or
+ *                k_norm (fp32 [head_dim]); v is not normalised
+ *     q, k rotated at positions[t] as above; q_out, k_cache, v_cache as above
+ * in fp32 throughout, each stored value rounded once (le_rope_kv_cache_write
+ * rounds after its bias too). Negative slots, slots >= num_slots and positions
+ * outside [0, max_positions) as above. head_dim a multiple of 8 up to 512;
+ * qkv_row_stride a multiple of 8; qkv, bias, the norms, the tables, q_out and
+ * the caches 16-byte aligned (LE_EUNSUPPORTED otherwise). Buffers must not
+ * overlap; tokens of one call must not share a slot.
+ * ------------------------------------------------------------------------ */
+int le_qk_norm_rope_kv_cache_write(const void* qkv, le_dtype act_dtype, int64_t qkv_row_stride,
+                                   const float* bias, const float* q_norm, const float* k_norm,
+                                   float eps, const int32_t* positions, const int32_t* slot_mapping,
+                                   const float* cos_table, const float* sin_table, int max_positions,
+                                   int n_tokens, int q_heads, int kv_heads, int head_dim, void* q_out,
+                                   void* k_cache, void* v_cache, le_dtype cache_dtype,
+                                   int64_t num_slots, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
  * (3)(4) Paged attention, reference-shaped.
  * Replaces launch_attention_decode and launch_attention_decode_gqa
  * (cuda_kernels.h:50-64, attention_decode.cu:45-161,
@@ -275,6 +297,61 @@ int le_ragged_paged_attention_noalloc(const void* q, le_dtype act_dtype, const v
                                       const le_step_plan* plan, float scale, void* out, hipStream_t stream);
 
 /* ------------------------------------------------------------------------
+ * (3) Ragged paged attention of sequences that share their first blocks (no
+ * counterpart in the reference). Sequences whose tables begin with the same
+ * block ids (a common prompt in the scheduler's prefix cache) read these
+ * blocks once for all of them instead of once each: the packer finds the
+ * groups, the shared keys are attended by all rows of a group together on
+ * MFMA tiles, every sequence's own keys by its rows (decode rows, drafted
+ * tokens behind them, prefill chunks), and the parts are merged. A slice's
+ * blocks count as shared only up to its first row's, so all of them are
+ * computed before the step and seen by all of its rows.
+ * ------------------------------------------------------------------------ */
+typedef struct le_prefix_plan {
+  le_plan_config cfg;
+  int32_t n_tokens;   /* query rows, in the order of the slices */
+  int32_t n_slices;
+  int32_t n_groups;   /* groups of slices that share blocks */
+  int32_t n_items;    /* work items (per kv head) */
+  int32_t n_parts;    /* partial results of split rows */
+  int32_t reserved_;
+  int64_t saved_keys; /* cached rows that are not read again, summed over the groups */
+  /* byte offsets inside the packed buffer */
+  int64_t off_items, off_rows, off_ids, off_positions, off_part0, off_row_parts;
+  int64_t bytes;      /* total size of the packed buffer */
+  const void* dev;    /* device copy, set by le_prefix_plan_upload */
+} le_prefix_plan;
+
+/* Packs a step for le_shared_prefix_attention: the slices of le_plan_step
+ * (`tokens` and `needs_logits` are not read), and of cfg the shape, block size,
+ * kv_dtype and partition_tokens (0 = default); flags and table_capacity must be
+ * 0. Shared blocks of fewer than 64 keys are not taken together. LE_ENOSPACE
+ * with plan->bytes set if host_cap is too small. */
+int le_prefix_plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* cfg,
+                        void* host_buf, int64_t host_cap, le_prefix_plan* plan);
+
+/* One async copy of the packed buffer to dev_buf (16-byte aligned, >=
+ * plan->bytes), then plan->dev = dev_buf. The host buffer stays alive until
+ * the copy ends. */
+int le_prefix_plan_upload(le_prefix_plan* plan, const void* host_buf, void* dev_buf, hipStream_t stream);
+
+/* Bytes of workspace that a packed step needs (0: none). It needs no clearing;
+ * launches that share one must be ordered. */
+size_t le_shared_prefix_workspace_size(const le_prefix_plan* plan);
+
+/* out[t] for every row of the plan, as le_ragged_paged_attention on the same
+ * slices. The step's own K/V rows are in the cache already. With q and the
+ * cache of one 16-bit type the products are that type's (the softmax weights
+ * rounded to it, once or in two terms); with any other pair they are fp32. A
+ * block id outside [0, num_cache_blocks) reads as zeros. q, out and the caches
+ * 16-byte aligned (LE_EUNSUPPORTED otherwise). NaN or inf in a V row reaches
+ * rows before it of the same slice that share its tile of up to 128 columns. */
+int le_shared_prefix_attention(const void* q, le_dtype act_dtype, const void* k_cache,
+                               const void* v_cache, le_dtype kv_dtype, int64_t num_cache_blocks,
+                               const le_prefix_plan* plan, float scale, void* out, void* workspace,
+                               size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
  * (2)+(3) The scatter and the attention of a step in one call.
  * Equals le_kv_cache_write(k_new, v_new, new_dtype, <plan slots>, k_cache,
  * v_cache, kv_dtype, n_tokens, kv_heads*head_dim, num_cache_blocks*block_size)
@@ -363,6 +440,40 @@ int le_rope(void* x, le_dtype dtype, const int32_t* positions, const float* cos_
 int le_add_inplace(void* x, const void* y, le_dtype dtype, size_t n, hipStream_t stream);
 /* x[r][c] += bias[c], fp32 bias (launch_add_bias, cuda_kernels.h:38-39). */
 int le_add_bias(void* x, le_dtype dtype, const float* bias, int rows, int cols, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Verification of drafted tokens (speculative decoding), beside le_argmax_rows
+ * (no counterpart in the reference). Sequence s has the drafts
+ * draft_tokens[cu_drafts[s] .. cu_drafts[s + 1]) (none: it is only sampled) and
+ * one target row more than drafts, rows cu_drafts[s] + s .. of logits
+ * [n_drafts + n_seqs][logits_row_stride]; row j of it is what the target says
+ * in draft j's place. With p = softmax(row / temperature[s]) (NULL: 1), q the
+ * draft's probabilities (draft_probs [n_drafts][probs_row_stride], or NULL: the
+ * drafts were not sampled, q is 1 at the token):
+ *   draft j is accepted while accept_u[j] * q(x_j) < p(x_j);
+ *   the first rejected row gives a token from max(p - q, 0) (from p where that
+ *   is nothing), after the last draft the sequence's last row gives one from p:
+ *   the first token whose running mass exceeds sample_u[s] * the whole mass.
+ * A temperature of 0 or less (or NaN) is greedy: p is 1 at the row's first
+ * maximum. A logit that is NaN or -inf has probability 0, several of +inf share
+ * it; a row with nothing above -inf has p 1 at token 0. A draft outside
+ * [0, vocab) is rejected. Random numbers are in [0, 1); 1 or more, or NaN, never
+ * accepts, and samples the last token with any mass. Sums and comparisons are
+ * fp64 over fp32 weights.
+ * out[s] = [accepted drafts..., the sampled token, -1...], max_drafts + 1
+ * entries; n_accepted[s] the number of accepted drafts. Offsets that decrease,
+ * leave [0, n_drafts] or hold more than max_drafts give out[s] = -1... and
+ * n_accepted[s] = -1. Rows may start at any element; the workspace is 16-byte
+ * aligned, needs no clearing, and is used by one call at a time.
+ * ------------------------------------------------------------------------ */
+size_t le_verify_drafts_workspace_size(int n_seqs, int n_drafts, int vocab);
+
+int le_verify_drafts(const void* logits, le_dtype logits_dtype, int64_t logits_row_stride, int vocab,
+                     const void* draft_probs, le_dtype probs_dtype, int64_t probs_row_stride,
+                     const int32_t* cu_drafts, const int32_t* draft_tokens, const float* accept_u,
+                     const float* sample_u, const float* temperature, int n_seqs, int n_drafts,
+                     int max_drafts, int32_t* out, int32_t* n_accepted, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

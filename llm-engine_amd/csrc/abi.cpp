@@ -5,6 +5,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 #include <mutex>
 #include <cstring>
 
@@ -15,15 +16,8 @@
 #define LE_VERSION_STRING "llm-engine-amd 0.1 (gfx950)"
 #endif
 
-namespace {
+namespace le {
 
-int hip_status(hipError_t e) { return e == hipSuccess ? LE_OK : static_cast<int>(e); }
-
-bool valid_dtype(int d) { return d == LE_F32 || d == LE_BF16 || d == LE_F16; }
-
-bool pow2(int x) { return x > 0 && (x & (x - 1)) == 0; }
-
-// Shapes every attention kernel supports.
 int check_attention_shape(int q_heads, int kv_heads, int head_dim, int block_size) {
   if (q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || block_size <= 0) return LE_EINVAL;
   if (q_heads % kv_heads != 0) return LE_EINVAL;
@@ -31,8 +25,24 @@ int check_attention_shape(int q_heads, int kv_heads, int head_dim, int block_siz
   if (head_dim != 64 && head_dim != 128) return LE_EUNSUPPORTED;
   // The score buffer holds 512 positions, a whole number of blocks; a wave
   // load covers up to 8 rows of a block.
-  if (!pow2(block_size) || block_size < 8 || block_size > 512) return LE_EUNSUPPORTED;
+  if ((block_size & (block_size - 1)) != 0 || block_size < 8 || block_size > 512) return LE_EUNSUPPORTED;
   return LE_OK;
+}
+
+}  // namespace le
+
+namespace {
+
+using le::check_attention_shape;
+
+int hip_status(hipError_t e) { return e == hipSuccess ? LE_OK : static_cast<int>(e); }
+
+bool valid_dtype(int d) { return d == LE_F32 || d == LE_BF16 || d == LE_F16; }
+
+bool aligned16(std::initializer_list<const void*> ptrs) {
+  for (const void* q : ptrs)
+    if (reinterpret_cast<uintptr_t>(q) & 15) return false;
+  return true;
 }
 
 size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
@@ -117,6 +127,113 @@ int le_rope_kv_cache_write(const void* qkv, le_dtype act_dtype, int64_t qkv_row_
   return hip_status(le::rope_kv_cache_write(qkv, act_dtype, qkv_row_stride, bias, positions, slot_mapping,
                                             cos_table, sin_table, max_positions, n_tokens, q_heads, kv_heads,
                                             head_dim, q_out, k_cache, v_cache, cache_dtype, num_slots, stream));
+}
+
+int le_qk_norm_rope_kv_cache_write(const void* qkv, le_dtype act_dtype, int64_t qkv_row_stride,
+                                   const float* bias, const float* q_norm, const float* k_norm,
+                                   float eps, const int32_t* positions, const int32_t* slot_mapping,
+                                   const float* cos_table, const float* sin_table, int max_positions,
+                                   int n_tokens, int q_heads, int kv_heads, int head_dim, void* q_out,
+                                   void* k_cache, void* v_cache, le_dtype cache_dtype,
+                                   int64_t num_slots, hipStream_t stream) {
+  if (n_tokens < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || num_slots < 0 ||
+      max_positions <= 0 || !(eps >= 0.f) || !std::isfinite(eps))
+    return LE_EINVAL;
+  if (!valid_dtype(act_dtype) || !valid_dtype(cache_dtype)) return LE_EINVAL;
+  if (head_dim % 8 != 0 || head_dim > 512) return LE_EUNSUPPORTED;
+  const int64_t row = (static_cast<int64_t>(q_heads) + 2 * static_cast<int64_t>(kv_heads)) * head_dim;
+  if (row > INT32_MAX) return LE_EUNSUPPORTED;
+  if (qkv_row_stride < row) return LE_EINVAL;
+  if (qkv_row_stride % 8 != 0) return LE_EUNSUPPORTED;  // 16-byte vector rows
+  if (n_tokens == 0) return LE_OK;
+  if (!qkv || !q_norm || !k_norm || !positions || !slot_mapping || !cos_table || !sin_table || !q_out ||
+      !k_cache || !v_cache)
+    return LE_EINVAL;
+  if (!aligned16({qkv, bias, q_norm, k_norm, cos_table, sin_table, q_out, k_cache, v_cache})) return LE_EUNSUPPORTED;
+  le::QkNormParams p{};
+  p.qkv = qkv; p.row_stride = qkv_row_stride; p.bias = bias;
+  p.q_norm = q_norm; p.k_norm = k_norm; p.eps = eps;
+  p.positions = positions; p.slots = slot_mapping; p.cos_t = cos_table; p.sin_t = sin_table;
+  p.max_pos = max_positions; p.n_tokens = n_tokens;
+  p.q_heads = q_heads; p.kv_heads = kv_heads; p.head_dim = head_dim;
+  p.q_out = q_out; p.k_cache = k_cache; p.v_cache = v_cache; p.num_slots = num_slots;
+  return hip_status(le::qk_norm_rope_kv_write(p, act_dtype, cache_dtype, stream));
+}
+
+size_t le_verify_drafts_workspace_size(int n_seqs, int n_drafts, int vocab) {
+  if (n_seqs <= 0 || n_drafts < 0 || vocab <= 0) return 0;
+  return le::verify_workspace(n_seqs, n_drafts, vocab);
+}
+
+int le_verify_drafts(const void* logits, le_dtype logits_dtype, int64_t logits_row_stride, int vocab,
+                     const void* draft_probs, le_dtype probs_dtype, int64_t probs_row_stride,
+                     const int32_t* cu_drafts, const int32_t* draft_tokens, const float* accept_u,
+                     const float* sample_u, const float* temperature, int n_seqs, int n_drafts,
+                     int max_drafts, int32_t* out, int32_t* n_accepted, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream) {
+  if (n_seqs < 0 || n_drafts < 0 || max_drafts < 0 || vocab <= 0) return LE_EINVAL;
+  if (!valid_dtype(logits_dtype) || (draft_probs && !valid_dtype(probs_dtype))) return LE_EINVAL;
+  if (logits_row_stride < vocab || (draft_probs && probs_row_stride < vocab)) return LE_EINVAL;
+  // grid dimensions, and token indices in 32 bits
+  if (n_seqs > 65535 || max_drafts > 65534 || vocab > INT32_MAX - le::kVerifyPiece) return LE_EUNSUPPORTED;
+  if (n_seqs == 0) return LE_OK;
+  if (!logits || !cu_drafts || !sample_u || !out || !n_accepted) return LE_EINVAL;
+  if (n_drafts > 0 && (!draft_tokens || !accept_u)) return LE_EINVAL;
+  if (!workspace || workspace_bytes < le_verify_drafts_workspace_size(n_seqs, n_drafts, vocab)) return LE_ENOSPACE;
+  if (!aligned16({workspace})) return LE_EUNSUPPORTED;
+  le::VerifyParams p{};
+  p.logits = logits; p.logits_stride = logits_row_stride; p.vocab = vocab;
+  p.draft_probs = draft_probs; p.probs_stride = probs_row_stride;
+  p.cu_drafts = cu_drafts; p.draft_tokens = draft_tokens;
+  p.accept_u = accept_u; p.sample_u = sample_u; p.temperature = temperature;
+  p.n_seqs = n_seqs; p.n_drafts = n_drafts; p.max_drafts = max_drafts;
+  p.out = out; p.n_accepted = n_accepted;
+  return hip_status(le::verify_drafts(p, logits_dtype, draft_probs ? probs_dtype : LE_F32, workspace, stream));
+}
+
+size_t le_shared_prefix_workspace_size(const le_prefix_plan* plan) {
+  if (!plan || plan->n_parts <= 0) return 0;
+  const size_t rows = static_cast<size_t>(plan->n_parts) * plan->cfg.q_heads;
+  return align256(rows * plan->cfg.head_dim * sizeof(float)) + align256(rows * sizeof(float2));
+}
+
+int le_shared_prefix_attention(const void* q, le_dtype act_dtype, const void* k_cache, const void* v_cache,
+                               le_dtype kv_dtype, int64_t num_cache_blocks, const le_prefix_plan* plan,
+                               float scale, void* out, void* workspace, size_t workspace_bytes,
+                               hipStream_t stream) {
+  if (!plan || !valid_dtype(act_dtype) || !valid_dtype(kv_dtype)) return LE_EINVAL;
+  if (plan->n_tokens == 0) return LE_OK;
+  const le_plan_config& cfg = plan->cfg;
+  const int shape = check_attention_shape(cfg.q_heads, cfg.kv_heads, cfg.head_dim, cfg.block_size);
+  if (shape != LE_OK) return shape;
+  if (cfg.kv_dtype != kv_dtype) return LE_EINVAL;
+  if (!plan->dev || !q || !k_cache || !v_cache || !out || !std::isfinite(scale) || num_cache_blocks <= 0)
+    return LE_EINVAL;
+  if (cfg.kv_heads > 65535) return LE_EUNSUPPORTED;  // a grid dimension
+  if (!aligned16({q, k_cache, v_cache, out})) return LE_EUNSUPPORTED;
+  const size_t need = le_shared_prefix_workspace_size(plan);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return LE_ENOSPACE;
+  if (need > 0 && !aligned16({workspace})) return LE_EUNSUPPORTED;
+  const char* dev = static_cast<const char*>(plan->dev);
+  auto arr = [&](int64_t off) { return reinterpret_cast<const int32_t*>(dev + off); };
+  le::PrefixParams p{};
+  p.q = q; p.k_cache = k_cache; p.v_cache = v_cache; p.out = out;
+  p.items = reinterpret_cast<const le::PrefixItem*>(dev + plan->off_items);
+  p.rows = arr(plan->off_rows); p.ids = arr(plan->off_ids); p.positions = arr(plan->off_positions);
+  p.part0 = arr(plan->off_part0); p.row_parts = arr(plan->off_row_parts);
+  if (need > 0) {
+    p.acc = static_cast<float*>(workspace);
+    p.ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) +
+                                     align256(static_cast<size_t>(plan->n_parts) * cfg.q_heads * cfg.head_dim * sizeof(float)));
+  }
+  p.n_items = plan->n_items; p.n_tokens = plan->n_tokens; p.n_parts = plan->n_parts;
+  p.q_heads = cfg.q_heads; p.kv_heads = cfg.kv_heads; p.head_dim = cfg.head_dim; p.block_size = cfg.block_size;
+  // the kernel's running maximum wants a positive factor; one of 0 becomes so
+  // small that every score is 0 (and a masked one stays -inf)
+  p.negate = scale < 0.f;
+  p.scale_log2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 1.1754944e-38f);
+  p.num_cache_blocks = num_cache_blocks;
+  return hip_status(le::attention_prefix(p, act_dtype, kv_dtype, stream));
 }
 
 size_t le_attention_decode_workspace_size(int n_tokens, int q_heads, int kv_heads, int head_dim) {

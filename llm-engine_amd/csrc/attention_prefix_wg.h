@@ -1,0 +1,609 @@
+#pragma once
+// Attention of sequences that share a prefix, over the paged cache: the
+// workgroup of one work item, and the merge of split rows.
+//
+// An item (PrefixItem, le_internal.h) is a tile of query columns (row, head of
+// one kv head) against a range of keys of one block table: the shared keys,
+// attended by the rows of every sequence of a group, or the keys that follow
+// them, by one sequence's rows under the causal mask. For a column c
+//     s_k = q_c . k_k scale,  m = max_k s_k,  l = sum_k e^(s_k - m),
+//     o = sum_k e^(s_k - m) v_k
+// over the item's keys; a row with one item is done (out = o / l), the others
+// leave (m, l, o) in fp32 and the merge adds them up:
+//     out = sum_i o_i e^(m_i - M) / sum_i l_i e^(m_i - M),  M = max_i m_i.
+//
+// Four waves load 64 keys at a time into LDS (double buffered, the next
+// tile's loads in registers meanwhile) and share them in one of two ways:
+//   * tiles of more than 32 columns: a wave has 32 columns and all 64 keys
+//     (32x32x16 MFMA);
+//   * up to 32 columns, where three waves would idle: a wave has all columns
+//     and 16 of the 64 keys (16x16 MFMAs), and the four waves' (m, l, o) are
+//     merged at the end. A single row is this case: it is bound by its keys'
+//     bytes, not by the products.
+// S^T = K Q^T and O^T = V^T P^T: a lane holds one column, and its scores are
+// the second product's B operand as they are (A and B only have to agree on
+// the order of keys). q enters as it is and the scale is applied to the fp32
+// scores, so 16-bit products are exact.
+//
+// Arithmetic: q, K and V of one 16-bit type use that type's MFMA, and the
+// softmax weights are rounded to it (the row sum is of the rounded weights; in
+// the key-sharing case, which has the matrix cores to spare, they are two
+// 16-bit terms instead). Anything else (fp32 activations or an fp32 cache)
+// uses the fp32 MFMA on widened operands.
+#include <float.h>
+
+#include <type_traits>
+
+#include "le_common.h"
+#include "le_internal.h"
+
+namespace le {
+namespace pfx {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kKeys = kPrefixTileKeys;  // keys of an LDS tile
+constexpr int kNarrow = 32;             // columns up to which the waves share keys
+constexpr float kSlack = 8.f;           // log2 units that scores may pass a column's base by
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef short bf16raw4 __attribute__((ext_vector_type(4)));
+
+// The operand type: the 16-bit type of both, or float.
+template <typename ACT, typename KV>
+using operand = std::conditional_t<std::is_same_v<ACT, KV> && sizeof(KV) == 2, KV, float>;
+
+// Products over 16 (wide: 32x32 tiles) or 32 (narrow: 16x16 tiles) dims, a
+// lane holding eight consecutive ones of its row of A and column of B; and
+// over keys, four of a lane's scores at a time (nt) or eight (wt).
+template <typename X> struct mm;
+template <> struct mm<bf16_t> {
+  using frag = bf16x8;
+  using scalar = __bf16;
+  __device__ __forceinline__ static frag load(const char* p) { return *reinterpret_cast<const frag*>(p); }
+  __device__ __forceinline__ static f32x16 wide(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static f32x4 narrow(frag a, frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static f32x4 keys16(bf16x4 a, bf16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16raw4, a), __builtin_bit_cast(bf16raw4, b),
+                                                     c, 0, 0, 0);
+  }
+};
+template <> struct mm<f16_t> {
+  using frag = f16x8;
+  using scalar = _Float16;
+  __device__ __forceinline__ static frag load(const char* p) { return *reinterpret_cast<const frag*>(p); }
+  __device__ __forceinline__ static f32x16 wide(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static f32x4 narrow(frag a, frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  __device__ __forceinline__ static f32x4 keys16(f16x4 a, f16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct mm<float> {
+  using frag = f32x8;
+  using scalar = float;
+  __device__ __forceinline__ static f32x16 wide(const frag& a, const frag& b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  __device__ __forceinline__ static f32x4 narrow(const frag& a, const frag& b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// Rows of the LDS tile, padded: K by 16 bytes (16-byte fragment reads of
+// consecutive rows cover all banks), V by 32 (so do the transposing reads).
+template <typename KV, int HD> struct Tile {
+  static constexpr int KROW = HD * static_cast<int>(sizeof(KV)) + 16;
+  static constexpr int VROW = HD * static_cast<int>(sizeof(KV)) + 32;
+  static constexpr int K_BYTES = kKeys * KROW;
+  static constexpr int BYTES = kKeys * (KROW + VROW);
+};
+template <typename KV, int HD> struct Smem {
+  __attribute__((aligned(16))) char lds[2 * Tile<KV, HD>::BYTES];
+  float2 ml[kWaves][kNarrow];  // a wave's (max, sum) of each column, at the end
+};
+// the end's accumulators of the four waves, in the tiles' place
+template <int HD> constexpr int kAccRow = HD + 4;
+
+// eight elements of an LDS row as an operand
+template <typename X, typename KV> __device__ __forceinline__ typename mm<X>::frag lds_frag(const char* p) {
+  if constexpr (std::is_same_v<X, float>) {
+    float f[8];
+    elem<KV>::load8(reinterpret_cast<const KV*>(p), f);
+    f32x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; e++) r[e] = f[e];
+    return r;
+  } else {
+    return mm<X>::load(p);
+  }
+}
+
+__device__ __forceinline__ float halves_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return vmax2(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// A query column: its row's token and head, and the last key that it sees,
+// relative to the item's first (negative: none of them).
+struct Column {
+  int token, head, lim;
+  bool ok;  // the column exists
+};
+__device__ __forceinline__ Column column_of(const PrefixParams& p, const PrefixItem& it, int kvh, int c) {
+  const int G = p.q_heads / p.kv_heads;
+  const int r = c / G;
+  Column o;
+  const bool ok = r < it.n_rows;
+  o.ok = ok;
+  o.token = p.rows[it.rows_off + (ok ? r : 0)];
+  o.head = kvh * G + (ok ? c - r * G : 0);
+  o.lim = ok ? min(it.key_end - 1, p.positions[o.token]) - it.key_begin : -1;
+  return o;
+}
+
+// eight elements of a column's q from dim d on, with the scale's sign
+template <typename ACT, typename X>
+__device__ __forceinline__ typename mm<X>::frag q_frag(const PrefixParams& p, const Column& c, int hd, int d) {
+  float f[8];
+  elem<ACT>::load8(static_cast<const ACT*>(p.q) + (static_cast<int64_t>(c.token) * p.q_heads + c.head) * hd + d, f);
+  typename mm<X>::frag r;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const float x = c.lim >= 0 ? (p.negate ? -f[e] : f[e]) : 0.f;
+    r[e] = static_cast<typename mm<X>::scalar>(x);
+  }
+  return r;
+}
+
+// Where a row's part is written: its record's accumulator and (m, l).
+__device__ __forceinline__ int64_t record_of(const PrefixParams& p, const PrefixItem& it, const Column& c) {
+  return (static_cast<int64_t>(p.part0[c.token]) + it.part) * p.q_heads + c.head;
+}
+
+// Keys of a tile, moved by all threads: a thread has one 16-byte piece of
+// KPT keys' K and V rows.
+template <typename KV, int HD> struct Loader {
+  static constexpr int CPR = HD * static_cast<int>(sizeof(KV)) / 16;
+  static constexpr int KPT = kKeys * CPR / kThreads;
+  static constexpr int KSTEP = kThreads / CPR;
+  using L = Tile<KV, HD>;
+  const char* kbase;
+  const char* vbase;
+  const int32_t* ids;
+  int64_t row_bytes, num_blocks;
+  int n_keys, key_l, piece, bs_shift, bs_mask;
+  int32_t bid[KPT];
+  uint4 k[KPT], v[KPT];
+  bool ok[KPT];
+
+  __device__ __forceinline__ Loader(const PrefixParams& p, const PrefixItem& it, int kvh) {
+    constexpr int HB = HD * static_cast<int>(sizeof(KV));
+    kbase = static_cast<const char*>(p.k_cache) + static_cast<int64_t>(kvh) * HB;
+    vbase = static_cast<const char*>(p.v_cache) + static_cast<int64_t>(kvh) * HB;
+    ids = p.ids + it.ids_off;
+    row_bytes = static_cast<int64_t>(p.kv_heads) * HB;
+    num_blocks = p.num_cache_blocks;
+    n_keys = it.key_end - it.key_begin;
+    key_l = threadIdx.x / CPR;
+    piece = threadIdx.x - key_l * CPR;
+    bs_shift = __builtin_ctz(p.block_size);
+    bs_mask = p.block_size - 1;
+  }
+  __device__ __forceinline__ void fetch_ids(int rel0) {
+#pragma unroll
+    for (int i = 0; i < KPT; i++) bid[i] = ids[min(rel0 + key_l + i * KSTEP, n_keys - 1) >> bs_shift];
+  }
+  __device__ __forceinline__ void issue(int rel0) {
+#pragma unroll
+    for (int i = 0; i < KPT; i++) {
+      const int rel = rel0 + key_l + i * KSTEP;
+      const bool in = bid[i] >= 0 && bid[i] < num_blocks;
+      ok[i] = in && rel < n_keys;
+      const int64_t off =
+          ((static_cast<int64_t>(in ? bid[i] : 0) << bs_shift) + (min(rel, n_keys - 1) & bs_mask)) * row_bytes + piece * 16;
+      k[i] = ld16(kbase + off);
+      v[i] = ld16(vbase + off);
+    }
+  }
+  // keys past the range, and blocks outside the cache, become zeros
+  __device__ __forceinline__ void stash(char* b) const {
+#pragma unroll
+    for (int i = 0; i < KPT; i++) {
+      const int key = key_l + i * KSTEP;
+      *reinterpret_cast<uint4*>(b + key * L::KROW + piece * 16) = ok[i] ? k[i] : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(b + L::K_BYTES + key * L::VROW + piece * 16) = ok[i] ? v[i] : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+// ---- more than 32 columns: 32 a wave ----
+template <typename ACT, typename KV, int HD>
+__device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixItem& it, int kvh, Smem<KV, HD>& sm) {
+  using X = operand<ACT, KV>;
+  using M = mm<X>;
+  using L = Tile<KV, HD>;
+  constexpr int KS = HD / 16, DT = HD / 32, U = kKeys / 32;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int col = lane & 31, half = lane >> 5, l16 = lane & 15;
+  Loader<KV, HD> ld(p, it, kvh);
+  ld.fetch_ids(0);
+  const Column c = column_of(p, it, kvh, wave * 32 + col);
+  typename M::frag qb[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) qb[ks] = q_frag<ACT, X>(p, c, HD, ks * 16 + half * 8);
+  ld.issue(0);
+  ld.fetch_ids(kKeys);
+  // the wave's keys: none past the last one that any of its columns sees, and
+  // no mask up to the first that one does not (columns without a row aside)
+  const int G = p.q_heads / p.kv_heads;
+  const bool any = wave * 32 / G < it.n_rows;
+  int wave_lim = c.lim, free_lim = c.ok ? c.lim : INT32_MAX;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    wave_lim = max(wave_lim, __shfl_xor(wave_lim, d, kWave));
+    free_lim = min(free_lim, __shfl_xor(free_lim, d, kWave));
+  }
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[d][e] = 0.f;
+  float base = 0.f, thr = -FLT_MAX, lsum = 0.f;  // thr -FLT_MAX: no key yet
+  const float scale = p.scale_log2;
+  const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
+  ld.stash(sm.lds);
+  __syncthreads();
+  for (int t = 0; t < n_tiles; t++) {
+    const int rel = t * kKeys;
+    if (t + 1 < n_tiles) {
+      ld.issue(rel + kKeys);
+      ld.fetch_ids(rel + 2 * kKeys);
+    }
+    const char* b = sm.lds + (t & 1) * L::BYTES;
+    if (any && rel <= wave_lim) {
+      f32x16 s[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[u][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+          s[u] = M::wide(lds_frag<X, KV>(b + (u * 32 + col) * L::KROW + (ks * 16 + half * 8) * static_cast<int>(sizeof(KV))),
+                         qb[ks], s[u]);
+      }
+      // accumulator e of a lane is key 8 (e / 4) + 4 half + e % 4
+      if (rel + kKeys - 1 > free_lim) {
+        const int m = c.lim - rel - half * 4;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (32 * u + 8 * (e / 4) + e % 4 > m) s[u][e] = -INFINITY;
+      }
+      float mt = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) mt = vmax2(mt, s[u][e]);
+      const float y = __builtin_fmaf(mt, scale, -base);
+      if (__builtin_amdgcn_ballot_w64(y > thr)) {
+        // A column's first keys set its base to their maximum; later ones
+        // move it when they pass it by more than kSlack.
+        const float m = halves_max(y);
+        const bool go = m > thr;
+        const float shift = go ? m : 0.f;
+        const float alpha = go && thr != -FLT_MAX ? __builtin_amdgcn_exp2f(-shift) : 1.f;
+        base += shift;
+        thr = go ? kSlack : thr;
+        lsum *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; d++) acc[d] *= alpha;
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        if constexpr (std::is_same_v<X, float>) {
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            s[u][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -base));
+            lsum += s[u][e];
+          }
+          const char* vp = b + L::K_BYTES + (u * 32 + 4 * half) * L::VROW + col * static_cast<int>(sizeof(KV));
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+              const float a = elem<KV>::load1(reinterpret_cast<const KV*>(
+                  vp + (8 * (e / 4) + e % 4) * L::VROW + d * 32 * static_cast<int>(sizeof(KV))));
+              acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[u][e], acc[d], 0, 0, 0);
+            }
+        } else {
+          typename M::frag pb[2];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const auto w = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -base)));
+            pb[e / 8][e % 8] = w;
+            lsum += static_cast<float>(w);
+          }
+          // V^T operand of 16 keys: lane (dim 16 (lane / 16 % 2) + lane % 16,
+          // half) holds the keys of accumulators 8 h .. 8 h + 7
+          const char* vp = b + L::K_BYTES + (u * 32 + 4 * half + (l16 >> 2)) * L::VROW + ((lane >> 4) & 1) * 32 + (l16 & 3) * 8;
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+              const auto lo = lds_read_tr16<KV>(vp + 16 * h * L::VROW + d * 64);
+              const auto hi = lds_read_tr16<KV>(vp + (16 * h + 8) * L::VROW + d * 64);
+              const typename M::frag va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+              acc[d] = M::wide(va, pb[h], acc[d]);
+            }
+        }
+      }
+    }
+    if (t + 1 < n_tiles) {
+      ld.stash(sm.lds + ((t + 1) & 1) * L::BYTES);
+      __syncthreads();
+    }
+  }
+
+  // acc[d][e] = O[column][dim 32 d + 8 (e / 4) + 4 half + e % 4]
+  const float l = halves_sum(lsum);
+  if (!c.ok) return;
+  if (it.part < 0) {
+    ACT* out = static_cast<ACT*>(p.out) + (static_cast<int64_t>(c.token) * p.q_heads + c.head) * HD + half * 4;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const float f[4] = {acc[d][e] * inv, acc[d][e + 1] * inv, acc[d][e + 2] * inv, acc[d][e + 3] * inv};
+        elem<ACT>::store4(out + d * 32 + e * 2, f);
+      }
+    return;
+  }
+  const int64_t rec = record_of(p, it, c);
+  float* o = p.acc + rec * HD + half * 4;
+#pragma unroll
+  for (int d = 0; d < DT; d++)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<float4*>(o + d * 32 + e * 2) = make_float4(acc[d][e], acc[d][e + 1], acc[d][e + 2], acc[d][e + 3]);
+  if (half == 0) p.ml[rec] = make_float2(l > 0.f ? base : -FLT_MAX, l);
+}
+
+// ---- up to 32 columns: 16 of the 64 keys a wave ----
+// NC column tiles of 16, known at compile time: with a branch around the second
+// tile's products the compiler left the first one's result a wait too short on
+// the way past the branch (fp32: a score without its last product).
+template <typename ACT, typename KV, int HD, int NC>
+__device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixItem& it, int kvh, Smem<KV, HD>& sm) {
+  using X = operand<ACT, KV>;
+  using M = mm<X>;
+  using L = Tile<KV, HD>;
+  constexpr int KS = HD / 32, DT = HD / 16;
+  constexpr int ES = static_cast<int>(sizeof(KV));
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int l16 = lane & 15, g = lane >> 4;
+  const int G = p.q_heads / p.kv_heads;
+  Loader<KV, HD> ld(p, it, kvh);
+  ld.fetch_ids(0);
+  Column c[NC];
+  typename M::frag qb[NC][KS];
+#pragma unroll
+  for (int n = 0; n < NC; n++) {
+    c[n] = column_of(p, it, kvh, n * 16 + l16);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) qb[n][ks] = q_frag<ACT, X>(p, c[n], HD, ks * 32 + g * 8);
+  }
+  ld.issue(0);
+  ld.fetch_ids(kKeys);
+
+  f32x4 acc[NC][DT];
+  float m[NC], lsum[NC];
+#pragma unroll
+  for (int n = 0; n < NC; n++) {
+    m[n] = -FLT_MAX;
+    lsum[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; d++) acc[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float scale = p.scale_log2;
+  const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
+  ld.stash(sm.lds);
+  __syncthreads();
+  for (int t = 0; t < n_tiles; t++) {
+    const int rel = t * kKeys;
+    if (t + 1 < n_tiles) {
+      ld.issue(rel + kKeys);
+      ld.fetch_ids(rel + 2 * kKeys);
+    }
+    const int key0 = rel + wave * 16;  // this wave's keys
+    if (key0 < ld.n_keys) {
+      const char* b = sm.lds + (t & 1) * L::BYTES + wave * 16 * L::KROW;
+      const char* bv = sm.lds + (t & 1) * L::BYTES + L::K_BYTES + wave * 16 * L::VROW;
+      f32x4 s[NC];
+#pragma unroll
+      for (int n = 0; n < NC; n++) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        const auto ka = lds_frag<X, KV>(b + l16 * L::KROW + (ks * 32 + g * 8) * ES);
+#pragma unroll
+        for (int n = 0; n < NC; n++) s[n] = M::narrow(ka, qb[n][ks], s[n]);
+      }
+      // accumulator i of a lane is key 4 g + i
+      float w[NC][4];
+#pragma unroll
+      for (int n = 0; n < NC; n++) {
+        const int lim = c[n].lim - key0 - 4 * g;
+        float x[4], mt = -FLT_MAX;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          x[i] = i > lim ? -INFINITY : s[n][i] * scale;
+          mt = vmax2(mt, x[i]);
+        }
+        const float mn = vmax2(m[n], rows_max(mt));
+        if (__builtin_amdgcn_ballot_w64(mn > m[n])) {
+          const float alpha = __builtin_amdgcn_exp2f(m[n] - mn);
+          m[n] = mn;
+          lsum[n] *= alpha;
+#pragma unroll
+          for (int d = 0; d < DT; d++) acc[n][d] *= alpha;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          w[n][i] = __builtin_amdgcn_exp2f(x[i] - m[n]);
+          lsum[n] += w[n][i];
+        }
+      }
+      if constexpr (std::is_same_v<X, float>) {
+        const char* vp = bv + 4 * g * L::VROW + l16 * ES;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int d = 0; d < DT; d++) {
+            const float a = elem<KV>::load1(reinterpret_cast<const KV*>(vp + i * L::VROW + d * 16 * ES));
+#pragma unroll
+            for (int n = 0; n < NC; n++) acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, w[n][i], acc[n][d], 0, 0, 0);
+          }
+      } else {
+        typename mma16<KV>::v4 hi[NC], lo[NC];
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+  #pragma unroll
+          for (int i = 0; i < 4; i++) {
+            hi[n][i] = static_cast<typename M::scalar>(w[n][i]);
+            lo[n][i] = static_cast<typename M::scalar>(w[n][i] - static_cast<float>(hi[n][i]));
+          }
+        }
+        const char* vp = bv + (4 * g + (l16 >> 2)) * L::VROW + (l16 & 3) * 8;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+          const auto va = lds_read_tr16<KV>(vp + d * 32);
+#pragma unroll
+          for (int n = 0; n < NC; n++) {
+            acc[n][d] = M::keys16(va, hi[n], acc[n][d]);
+            acc[n][d] = M::keys16(va, lo[n], acc[n][d]);
+          }
+        }
+      }
+    }
+    if (t + 1 < n_tiles) {
+      ld.stash(sm.lds + ((t + 1) & 1) * L::BYTES);
+      __syncthreads();
+    }
+  }
+
+  // ---- the four waves' results, in the tiles' place ----
+  // acc[n][d][i] = O[column 16 n + l16][dim 16 d + 4 g + i]
+  constexpr int AR = kAccRow<HD>;
+  static_assert(kWaves * kNarrow * AR * 4 <= 2 * L::BYTES);
+  float* all = reinterpret_cast<float*>(sm.lds);
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NC; n++) {
+    const float l = rows_sum(lsum[n]);
+    if (g == 0) sm.ml[wave][n * 16 + l16] = make_float2(m[n], l);
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+      *reinterpret_cast<f32x4*>(all + (wave * kNarrow + n * 16 + l16) * AR + d * 16 + 4 * g) = acc[n][d];
+  }
+  __syncthreads();
+  constexpr int PIECES = HD / 4;
+  for (int i = threadIdx.x; i < it.n_rows * G * PIECES; i += kThreads) {
+    const int cc = i / PIECES, d = (i - cc * PIECES) * 4;
+    const Column o = column_of(p, it, kvh, cc);
+    float M4 = -FLT_MAX;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) M4 = fmaxf(M4, sm.ml[w][cc].x);
+    float l = 0.f;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      const float2 x = sm.ml[w][cc];
+      const float f = __builtin_amdgcn_exp2f(x.x - M4);
+      l += x.y * f;
+      a += *reinterpret_cast<const f32x4*>(all + (w * kNarrow + cc) * AR + d) * f;
+    }
+    if (it.part < 0) {
+      const float inv = 1.f / l;
+      const float f[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
+      elem<ACT>::store4(static_cast<ACT*>(p.out) + (static_cast<int64_t>(o.token) * p.q_heads + o.head) * HD + d, f);
+    } else {
+      const int64_t rec = record_of(p, it, o);
+      *reinterpret_cast<f32x4*>(p.acc + rec * HD + d) = a;
+      if (d == 0) p.ml[rec] = make_float2(M4, l);
+    }
+  }
+}
+
+template <typename ACT, typename KV, int HD>
+__global__ __launch_bounds__(kThreads, (std::is_same_v<operand<ACT, KV>, float> ? 1 : 2)) void prefix_kernel(PrefixParams p) {
+  __shared__ Smem<KV, HD> sm;
+  const PrefixItem it = p.items[blockIdx.x];
+  const int kvh = blockIdx.y;
+  const int cols = it.n_rows * (p.q_heads / p.kv_heads);
+  if (cols <= 16) narrow_item<ACT, KV, HD, 1>(p, it, kvh, sm);
+  else if (cols <= kNarrow) narrow_item<ACT, KV, HD, 2>(p, it, kvh, sm);
+  else wide_item<ACT, KV, HD>(p, it, kvh, sm);
+}
+
+// ---- rows of several parts: one thread per four dims of a (row, head) ----
+template <typename ACT, int HD>
+__global__ __launch_bounds__(kThreads) void prefix_merge_kernel(PrefixParams p) {
+  constexpr int PIECES = HD / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t rh = i / PIECES;
+  if (rh >= static_cast<int64_t>(p.n_tokens) * p.q_heads) return;
+  const int token = static_cast<int>(rh / p.q_heads), head = static_cast<int>(rh - static_cast<int64_t>(token) * p.q_heads);
+  const int d = static_cast<int>(i - rh * PIECES) * 4;
+  const int n = p.row_parts[token];
+  if (n <= 1) return;
+  const int64_t rec0 = static_cast<int64_t>(p.part0[token]) * p.q_heads + head;
+  float M = -FLT_MAX;
+  for (int k = 0; k < n; k++) M = fmaxf(M, p.ml[rec0 + static_cast<int64_t>(k) * p.q_heads].x);
+  float l = 0.f;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < n; k++) {
+    const int64_t rec = rec0 + static_cast<int64_t>(k) * p.q_heads;
+    const float2 x = p.ml[rec];
+    const float f = __builtin_amdgcn_exp2f(x.x - M);
+    l += x.y * f;
+    a += *reinterpret_cast<const f32x4*>(p.acc + rec * HD + d) * f;
+  }
+  const float inv = 1.f / l;
+  const float f[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
+  elem<ACT>::store4(static_cast<ACT*>(p.out) + rh * HD + d, f);
+}
+
+template <typename ACT, typename KV, int HD>
+hipError_t launch_prefix(const PrefixParams& p, hipStream_t stream) {
+  prefix_kernel<ACT, KV, HD><<<dim3(static_cast<unsigned>(p.n_items), static_cast<unsigned>(p.kv_heads)), kThreads, 0,
+                               stream>>>(p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.n_parts == 0) return e;
+  const int64_t threads = static_cast<int64_t>(p.n_tokens) * p.q_heads * (HD / 4);
+  prefix_merge_kernel<ACT, HD><<<static_cast<unsigned>((threads + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace pfx
+}  // namespace le

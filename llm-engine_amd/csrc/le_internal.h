@@ -8,6 +8,9 @@
 
 namespace le {
 
+// Shapes every attention kernel supports: LE_OK, or the code to return (abi.cpp).
+int check_attention_shape(int q_heads, int kv_heads, int head_dim, int block_size);
+
 // Split-K partial result of one (row, q head, context partition): the
 // unnormalised accumulator, and the running max (log2 domain) and sum.
 struct PartialLayout {
@@ -56,6 +59,83 @@ hipError_t rope_kv_cache_write(const void* qkv, int act_dtype, int64_t row_strid
                                int kv_heads, int head_dim, void* q_out, void* kc, void* vc,
                                int cache_dtype, int64_t num_slots, hipStream_t stream,
                                const void* rms_x = nullptr, int rms_hidden = 0, float rms_eps = 0.f);
+
+// Rows of the stacked QKV projection through per-head norms, RoPE and the
+// cache write (qk_norm_rope_kv_write.hip).
+struct QkNormParams {
+  const void* qkv;
+  int64_t row_stride;
+  const float* bias;    // [q | k | v], may be null
+  const float* q_norm;  // [head_dim] each
+  const float* k_norm;
+  float eps;
+  const int32_t* positions;
+  const int32_t* slots;
+  const float* cos_t;
+  const float* sin_t;
+  int max_pos, n_tokens, q_heads, kv_heads, head_dim;
+  int lanes;  // set by the launcher
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  int64_t num_slots;
+};
+hipError_t qk_norm_rope_kv_write(const QkNormParams& p, int act_dtype, int cache_dtype, hipStream_t stream);
+
+// Verification of drafted tokens (verify_drafts.hip).
+constexpr int kVerifyPiece = 2048;  // tokens of a row that one wave takes
+struct VerifyParams {
+  const void* logits;       // [n_drafts + n_seqs][logits_stride]: sequence s's rows from cu_drafts[s] + s on
+  int64_t logits_stride;
+  const void* draft_probs;  // [n_drafts][probs_stride], or null
+  int64_t probs_stride;
+  const int32_t* cu_drafts;
+  const int32_t* draft_tokens;
+  const float* accept_u;
+  const float* sample_u;
+  const float* temperature;  // null: 1
+  int n_seqs, n_drafts, max_drafts, vocab;
+  int32_t* out;              // [n_seqs][max_drafts + 1]
+  int32_t* n_accepted;
+  // set by the launcher
+  int n_pieces;
+  void* choices;
+  void* stats;
+  double* mass;
+};
+size_t verify_workspace(int64_t n_seqs, int64_t n_drafts, int vocab);
+hipError_t verify_drafts(const VerifyParams& p, int logits_dtype, int probs_dtype, void* workspace, hipStream_t stream);
+
+// Shared-prefix attention (attention_prefix_wg.h). A work item: the query rows
+// rows[rows_off .. + n_rows) (token indices) against keys [key_begin, key_end)
+// of the table whose block ids, from key_begin's block on, are at ids_off.
+// part: which of its rows' parts this is; -1: their only one, written out.
+// causal: rows see keys up to their own position.
+struct PrefixItem {
+  int32_t rows_off, n_rows, ids_off, key_begin, key_end, part, causal, reserved;
+};
+constexpr int kPrefixCols = 128;     // query columns (row, head) of an item, at most
+constexpr int kPrefixTileKeys = 64;  // keys of an LDS tile: partitions are whole tiles
+struct PrefixParams {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* out;
+  const PrefixItem* items;
+  const int32_t* rows;
+  const int32_t* ids;
+  const int32_t* positions;  // of every token
+  const int32_t* part0;      // a token's first record; its parts' follow
+  const int32_t* row_parts;  // its number of parts
+  float* acc;                // [records][q_heads][head_dim] unnormalised
+  float2* ml;                // [records][q_heads] (max in log2 units, sum)
+  int n_items, n_tokens, n_parts, q_heads, kv_heads, head_dim, block_size;
+  float scale_log2;          // > 0
+  int negate;                // the scale was negative: q changes its sign
+  int64_t num_cache_blocks;
+};
+hipError_t attention_prefix(const PrefixParams& p, int act_dtype, int kv_dtype, hipStream_t stream);
+hipError_t attention_prefix_f32(const PrefixParams& p, int act_dtype, int kv_dtype, hipStream_t stream);
 
 struct DecodeParams {
   const void* q;

@@ -1,0 +1,302 @@
+// Packing of a step for shared-prefix attention: le_prefix_plan_step /
+// le_prefix_plan_upload.
+//
+// Sequences whose block tables begin with the same ids (the scheduler's prefix
+// cache hands one prompt's blocks to all of them) share those keys. The
+// tables, each cut where its sequence's own rows begin, are sorted; runs with
+// a common beginning form a tree (their longest common prefixes are nested),
+// and the groups are the cut through it that saves the most block reads. A
+// group's shared keys are attended by all rows of its sequences at once, in
+// tiles of query columns (row, head); what follows them by each sequence's
+// rows alone. Every tile's keys are cut into partitions, one work item each.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstring>
+#include <new>
+#include <unordered_map>
+#include <vector>
+
+#include "le_internal.h"
+#include "llm_engine_amd.h"
+
+namespace {
+
+using le::PrefixItem;
+
+constexpr int kMinSharedKeys = 64;    // a shorter common beginning is not worth a pass of its own
+constexpr int64_t kTargetWorkgroups = 512;  // two per CU
+constexpr int kMinPart = 128;         // keys of the shortest partition
+constexpr int kMaxParts = 128;        // partitions of a tile
+
+int64_t align256(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
+
+struct Group {
+  int first, count;  // among the sorted slices
+  int blocks;        // shared blocks
+};
+
+// The groups of sorted tables with common beginnings lcp[i] (of i - 1 and i).
+// One pass with a stack of open runs; a closed run is worth its shared blocks
+// times the sequences that need not read them, or what its inner runs are.
+std::vector<Group> best_groups(const std::vector<int>& lcp, int min_blocks) {
+  struct Run {
+    int v, first, last;
+    int64_t best;
+    bool whole;
+    std::vector<int> inner;
+  };
+  const int n = static_cast<int>(lcp.size());
+  std::vector<Run> runs;  // closed ones, inner before outer
+  std::vector<Run> open{Run{0, 0, 0, 0, false, {}}};
+  for (int i = 1; i <= n; i++) {
+    const int v = i < n ? lcp[i] : 0;
+    int first = i - 1, closed = -1;
+    while (v < open.back().v) {
+      Run r = std::move(open.back());
+      open.pop_back();
+      r.last = i - 1;
+      int64_t inside = 0;
+      for (int k : r.inner) inside += runs[k].best;
+      const int64_t all = r.v >= min_blocks ? static_cast<int64_t>(r.v) * (r.last - r.first) : 0;
+      r.whole = all > 0 && all >= inside;
+      r.best = std::max(all, inside);
+      first = r.first;
+      closed = static_cast<int>(runs.size());
+      runs.push_back(std::move(r));
+      if (v <= open.back().v) {
+        open.back().inner.push_back(closed);
+        closed = -1;
+      }
+    }
+    if (v > open.back().v) {
+      Run r{v, first, 0, 0, false, {}};
+      if (closed >= 0) r.inner.push_back(closed);
+      open.push_back(std::move(r));
+    }
+  }
+  std::vector<Group> groups;
+  std::vector<int> todo = open.front().inner;
+  while (!todo.empty()) {
+    const Run& r = runs[todo.back()];
+    todo.pop_back();
+    if (r.whole) groups.push_back(Group{r.first, r.last - r.first + 1, r.v});
+    else todo.insert(todo.end(), r.inner.begin(), r.inner.end());
+  }
+  return groups;
+}
+
+struct Tile {
+  std::vector<int32_t> rows;
+  int32_t ids_off;  // block id of key_begin
+  int32_t key_begin, key_end;
+  bool causal;
+  int part_first;  // index of its first partition among those of its rows
+  int parts;
+};
+
+int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* cfg_in, void* host_buf,
+              int64_t host_cap, le_prefix_plan* plan) {
+  if (!plan || !cfg_in || n_slices < 0 || (n_slices > 0 && !slices)) return LE_EINVAL;
+  const le_plan_config& cfg = *cfg_in;
+  const int shape = le::check_attention_shape(cfg.q_heads, cfg.kv_heads, cfg.head_dim, cfg.block_size);
+  if (shape != LE_OK) return shape;
+  if (cfg.kv_dtype != LE_F32 && cfg.kv_dtype != LE_BF16 && cfg.kv_dtype != LE_F16) return LE_EINVAL;
+  if (cfg.partition_tokens < 0 || cfg.flags != 0 || cfg.table_capacity != 0) return LE_EINVAL;
+  const int bs = cfg.block_size, G = cfg.q_heads / cfg.kv_heads;
+
+  // ---- validation; a key's slices use its first one's table, as le_plan_step's do ----
+  int64_t n_tok = 0;
+  std::unordered_map<int64_t, int> seen;
+  std::vector<const le_step_slice*> table(n_slices);
+  for (int i = 0; i < n_slices; i++) {
+    const le_step_slice& s = slices[i];
+    if (s.len <= 0 || s.start < 0 || s.num_blocks < 0 || s.len > INT32_MAX - s.start) return LE_EINVAL;
+    if (s.num_blocks > 0 && !s.blocks) return LE_EINVAL;
+    table[i] = &slices[seen.emplace(s.seq_key, i).first->second];
+    if ((s.start + s.len - 1) / bs >= table[i]->num_blocks) return LE_EINVAL;  // a position without a block
+    n_tok += s.len;
+  }
+  if (n_tok > INT32_MAX / 2) return LE_EUNSUPPORTED;
+  std::vector<int32_t> first_row(n_slices);
+  std::vector<int32_t> positions(static_cast<size_t>(n_tok));
+  for (int i = 0, t = 0; i < n_slices; i++) {
+    first_row[i] = t;
+    for (int j = 0; j < slices[i].len; j++) positions[t++] = slices[i].start + j;
+  }
+
+  // ---- groups ----
+  // whole blocks before a slice's first row: every key in them is visible to
+  // all its rows, and at least one key is left behind them
+  std::vector<int> cap(n_slices), order(n_slices);
+  for (int i = 0; i < n_slices; i++) {
+    cap[i] = slices[i].start / bs;
+    order[i] = i;
+  }
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) {
+    return std::lexicographical_compare(table[a]->blocks, table[a]->blocks + cap[a], table[b]->blocks,
+                                        table[b]->blocks + cap[b]);
+  });
+  std::vector<int> lcp(n_slices, 0);
+  for (int i = 1; i < n_slices; i++) {
+    const int a = order[i - 1], b = order[i], m = std::min(cap[a], cap[b]);
+    lcp[i] = static_cast<int>(
+        std::mismatch(table[a]->blocks, table[a]->blocks + m, table[b]->blocks).first - table[a]->blocks);
+  }
+  const std::vector<Group> groups = best_groups(lcp, std::max(1, (kMinSharedKeys + bs - 1) / bs));
+
+  // ---- tiles: shared keys by a group's rows, then every slice's own keys ----
+  std::vector<int32_t> ids;
+  std::vector<Tile> tiles;
+  std::vector<int> shared(n_slices, 0);       // keys of the slice that its group reads
+  const int tile_rows = le::kPrefixCols / G;
+  auto add_tiles = [&](const std::vector<int32_t>& rows, int32_t ids_off, int begin, bool causal, int end) {
+    const int n = static_cast<int>(rows.size());
+    const int count = (n + tile_rows - 1) / tile_rows;
+    for (int k = 0; k < count; k++) {
+      const int a = static_cast<int>(static_cast<int64_t>(k) * n / count);
+      const int b = static_cast<int>(static_cast<int64_t>(k + 1) * n / count);
+      // a causal tile's keys end with its last row's own
+      const int e = causal ? positions[rows[b - 1]] + 1 : end;
+      tiles.push_back(Tile{std::vector<int32_t>(rows.begin() + a, rows.begin() + b), ids_off, begin, e, causal, 0, 1});
+    }
+  };
+  for (size_t g = 0; g < groups.size(); g++) {
+    const Group& gr = groups[g];
+    std::vector<int32_t> rows;
+    for (int k = 0; k < gr.count; k++) {
+      const int i = order[gr.first + k];
+      shared[i] = gr.blocks * bs;
+      for (int j = 0; j < slices[i].len; j++) rows.push_back(first_row[i] + j);
+    }
+    std::sort(rows.begin(), rows.end());
+    const int32_t off = static_cast<int32_t>(ids.size());
+    const int32_t* t = table[order[gr.first]]->blocks;
+    ids.insert(ids.end(), t, t + gr.blocks);
+    add_tiles(rows, off, 0, false, gr.blocks * bs);
+  }
+  for (int i = 0; i < n_slices; i++) {
+    std::vector<int32_t> rows(slices[i].len);
+    for (int j = 0; j < slices[i].len; j++) rows[j] = first_row[i] + j;
+    const int32_t off = static_cast<int32_t>(ids.size());
+    const int b0 = shared[i] / bs, b1 = (slices[i].start + slices[i].len - 1) / bs + 1;
+    ids.insert(ids.end(), table[i]->blocks + b0, table[i]->blocks + b1);
+    add_tiles(rows, off, shared[i], true, 0);
+  }
+  if (ids.size() > INT32_MAX / 2) return LE_EUNSUPPORTED;
+
+  // ---- partitions ----
+  int64_t work = 0;
+  for (const Tile& t : tiles) work += static_cast<int64_t>(t.key_end - t.key_begin) * cfg.kv_heads;
+  const int quantum = std::max(le::kPrefixTileKeys, bs);
+  int64_t part = cfg.partition_tokens > 0 ? cfg.partition_tokens
+                                          : std::max<int64_t>(kMinPart, work / kTargetWorkgroups);
+  part = (part + quantum - 1) / quantum * quantum;
+  std::vector<int32_t> n_parts(static_cast<size_t>(n_tok), 0), part0(static_cast<size_t>(n_tok), 0);
+  int64_t n_items = 0, n_item_rows = 0;
+  for (Tile& t : tiles) {
+    const int64_t units = (t.key_end - t.key_begin + quantum - 1) / quantum;
+    t.parts = static_cast<int>(std::min<int64_t>(kMaxParts, (units * quantum + part - 1) / part));
+    t.part_first = n_parts[t.rows[0]];
+    for (int32_t r : t.rows) n_parts[r] += t.parts;
+    n_items += t.parts;
+    n_item_rows += static_cast<int64_t>(t.rows.size());
+  }
+  int64_t n_records = 0;
+  for (int64_t r = 0; r < n_tok; r++) {
+    part0[r] = static_cast<int32_t>(n_records);
+    if (n_parts[r] > 1) n_records += n_parts[r];
+  }
+  if (n_records > INT32_MAX / 2 || n_items > INT32_MAX / 2 || n_item_rows > INT32_MAX / 2) return LE_EUNSUPPORTED;
+
+  // ---- items, longest first ----
+  std::vector<PrefixItem> items;
+  items.reserve(static_cast<size_t>(n_items));
+  std::vector<int32_t> rows;
+  rows.reserve(static_cast<size_t>(n_item_rows));
+  for (const Tile& t : tiles) {
+    const int64_t units = (t.key_end - t.key_begin + quantum - 1) / quantum;
+    const int32_t off = static_cast<int32_t>(rows.size());
+    rows.insert(rows.end(), t.rows.begin(), t.rows.end());
+    const bool split = n_parts[t.rows[0]] > 1;
+    for (int k = 0; k < t.parts; k++) {
+      PrefixItem it{};
+      it.rows_off = off;
+      it.n_rows = static_cast<int32_t>(t.rows.size());
+      const int a = static_cast<int>(k * units / t.parts) * quantum, b = static_cast<int>((k + 1) * units / t.parts) * quantum;
+      it.key_begin = t.key_begin + a;
+      it.key_end = std::min<int64_t>(static_cast<int64_t>(t.key_begin) + b, t.key_end);
+      it.ids_off = t.ids_off + a / bs;
+      it.part = split ? t.part_first + k : -1;
+      it.causal = t.causal ? 1 : 0;
+      items.push_back(it);
+    }
+  }
+  std::stable_sort(items.begin(), items.end(), [](const PrefixItem& a, const PrefixItem& b) {
+    return a.key_end - a.key_begin > b.key_end - b.key_begin;
+  });
+
+  // ---- layout and copy ----
+  le_prefix_plan out{};
+  out.cfg = cfg;
+  out.n_tokens = static_cast<int32_t>(n_tok);
+  out.n_slices = n_slices;
+  out.n_groups = static_cast<int32_t>(groups.size());
+  out.n_items = static_cast<int32_t>(n_items);
+  out.n_parts = static_cast<int32_t>(n_records);
+  for (const Group& g : groups) out.saved_keys += static_cast<int64_t>(g.blocks) * bs * (g.count - 1);
+  int64_t at = 0;
+  auto place = [&](int64_t& off, size_t bytes) {
+    off = at;
+    at = align256(at + static_cast<int64_t>(bytes));
+  };
+  place(out.off_items, items.size() * sizeof(PrefixItem));
+  place(out.off_rows, rows.size() * 4);
+  place(out.off_ids, ids.size() * 4);
+  place(out.off_positions, positions.size() * 4);
+  place(out.off_part0, part0.size() * 4);
+  place(out.off_row_parts, n_parts.size() * 4);
+  out.bytes = at;
+  *plan = out;
+  if (out.bytes == 0) return LE_OK;
+  if (!host_buf || host_cap < out.bytes) return LE_ENOSPACE;
+  char* dst = static_cast<char*>(host_buf);
+  auto put = [&](int64_t off, const void* src, size_t bytes) {
+    if (bytes) std::memcpy(dst + off, src, bytes);
+  };
+  put(out.off_items, items.data(), items.size() * sizeof(PrefixItem));
+  put(out.off_rows, rows.data(), rows.size() * 4);
+  put(out.off_ids, ids.data(), ids.size() * 4);
+  put(out.off_positions, positions.data(), positions.size() * 4);
+  put(out.off_part0, part0.data(), part0.size() * 4);
+  put(out.off_row_parts, n_parts.data(), n_parts.size() * 4);
+  return LE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int le_prefix_plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* cfg, void* host_buf,
+                        int64_t host_cap, le_prefix_plan* plan) {
+  try {
+    return plan_step(slices, n_slices, cfg, host_buf, host_cap, plan);
+  } catch (...) {  // out of host memory
+    return LE_ENOSPACE;
+  }
+}
+
+int le_prefix_plan_upload(le_prefix_plan* plan, const void* host_buf, void* dev_buf, hipStream_t stream) {
+  if (!plan || plan->bytes < 0) return LE_EINVAL;
+  if (plan->bytes > 0) {
+    if (!host_buf || !dev_buf) return LE_EINVAL;
+    const hipError_t e =
+        hipMemcpyAsync(dev_buf, host_buf, static_cast<size_t>(plan->bytes), hipMemcpyHostToDevice, stream);
+    if (e != hipSuccess) return static_cast<int>(e);
+  }
+  plan->dev = dev_buf;
+  return LE_OK;
+}
+
+}  // extern "C"

@@ -88,6 +88,27 @@ class StepPlan(ctypes.Structure):
     ]
 
 
+class PrefixStepPlan(ctypes.Structure):
+    _fields_ = [
+        ("cfg", PlanConfig),
+        ("n_tokens", ctypes.c_int32),
+        ("n_slices", ctypes.c_int32),
+        ("n_groups", ctypes.c_int32),
+        ("n_items", ctypes.c_int32),
+        ("n_parts", ctypes.c_int32),
+        ("reserved_", ctypes.c_int32),
+        ("saved_keys", ctypes.c_int64),
+        ("off_items", ctypes.c_int64),
+        ("off_rows", ctypes.c_int64),
+        ("off_ids", ctypes.c_int64),
+        ("off_positions", ctypes.c_int64),
+        ("off_part0", ctypes.c_int64),
+        ("off_row_parts", ctypes.c_int64),
+        ("bytes", ctypes.c_int64),
+        ("dev", ctypes.c_void_p),
+    ]
+
+
 class SchedConfig(ctypes.Structure):
     _fields_ = [
         ("continuous", ctypes.c_int32),
@@ -149,6 +170,27 @@ SIGNATURES = {
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int,
         ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
         ctypes.c_int64, ctypes.c_void_p]),
+    "le_qk_norm_rope_kv_cache_write": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p]),
+    "le_verify_drafts_workspace_size": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "le_verify_drafts": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+        ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+        ctypes.c_void_p]),
+    "le_prefix_plan_step": (ctypes.c_int, [
+        ctypes.POINTER(StepSlice), ctypes.c_int, ctypes.POINTER(PlanConfig), ctypes.c_void_p,
+        ctypes.c_int64, ctypes.POINTER(PrefixStepPlan)]),
+    "le_prefix_plan_upload": (ctypes.c_int, [
+        ctypes.POINTER(PrefixStepPlan), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "le_shared_prefix_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(PrefixStepPlan)]),
+    "le_shared_prefix_attention": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+        ctypes.POINTER(PrefixStepPlan), ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+        ctypes.c_void_p]),
     "le_attention_decode_workspace_size": (ctypes.c_size_t, [
         ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "le_attention_decode": (ctypes.c_int, [

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import LE_BF16, LE_F16, LE_F32, PlanConfig, StepPlan, StepSlice, check
+from ._lib import LE_BF16, LE_F16, LE_F32, PlanConfig, PrefixStepPlan, StepPlan, StepSlice, check
 
 
 _DTYPES = {torch.float32: LE_F32, torch.bfloat16: LE_BF16, torch.float16: LE_F16}
@@ -46,6 +46,43 @@ def _dev_i32(t: torch.Tensor, name: str, n: int | None = None) -> None:
     _req(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{name}: contiguous int32 cuda tensor")
     if n is not None:
         _req(t.numel() >= n, f"{name}: needs {n} entries, has {t.numel()}")
+
+
+def _dev_f32(t: torch.Tensor, name: str, n: int | None = None) -> None:
+    _req(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous(), f"{name}: contiguous fp32 cuda tensor")
+    if n is not None:
+        _req(t.numel() == n, f"{name}: {n} entries, has {t.numel()}")
+
+
+def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    i = first.get_device()
+    for t in others:
+        _req(t is None or t.get_device() == i, "all tensors on one device")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements from row to row of a 2-d tensor; a single row's is its length
+    (whatever its stride says), rounded up to whole 16-byte pieces of any type."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+
+
+class _on:
+    """The tensors' device as the current one for the launch (the current
+    stream is then that device's); costs nothing where it already is."""
+
+    __slots__ = ("want", "was")
+
+    def __init__(self, device: torch.device):
+        self.want = device.index
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device()
+        if self.was != self.want:
+            torch.cuda.set_device(self.want)
+
+    def __exit__(self, *exc):
+        if self.was != self.want:
+            torch.cuda.set_device(self.was)
 
 
 def store_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
@@ -96,6 +133,47 @@ def rope_store_kv(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tenso
     return q_out
 
 
+def qk_norm_rope_store_kv(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, cos_t: torch.Tensor,
+                          sin_t: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float, q_heads: int,
+                          kv_heads: int, head_dim: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                          bias: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                          stream=None) -> torch.Tensor:
+    """rope_store_kv for models that normalise each q and k head before the
+    rotation: x / sqrt(mean(x^2) + eps) * q_norm or k_norm (fp32 [head_dim]),
+    after the bias, in fp32 with one rounding per stored value. Returns q:
+    [N, q_heads*head_dim]."""
+    _req(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.is_cuda, "qkv: cuda [N, row] with unit column stride")
+    n, row, kv_dim = qkv.shape[0], (q_heads + 2 * kv_heads) * head_dim, kv_heads * head_dim
+    _req(qkv.shape[1] >= row, "qkv rows too short")
+    _dev_f32(cos_t, "cos_t")
+    _dev_f32(sin_t, "sin_t")
+    _req(cos_t.shape == sin_t.shape and cos_t.dim() == 2 and cos_t.shape[1] == head_dim // 2,
+         "cos/sin: fp32 [max_pos, head_dim/2]")
+    _dev_f32(q_norm, "q_norm", head_dim)
+    _dev_f32(k_norm, "k_norm", head_dim)
+    _req(k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.is_contiguous()
+         and v_cache.is_contiguous() and k_cache.is_cuda and v_cache.is_cuda, "k/v caches must match and be contiguous")
+    num_slots = k_cache.shape[0]
+    _req(k_cache.numel() == num_slots * kv_dim, "cache row size must equal kv_dim")
+    _dev_i32(positions, "positions", n)
+    _dev_i32(slots, "slots", n)
+    if bias is not None:
+        _dev_f32(bias, "bias", row)
+    if q_out is None:
+        q_out = torch.empty(n, q_heads * head_dim, dtype=qkv.dtype, device=qkv.device)
+    _req(q_out.is_contiguous() and q_out.dtype == qkv.dtype and q_out.numel() == n * q_heads * head_dim
+         and q_out.is_cuda, "q_out: [N, q_heads*head_dim] in qkv's dtype")
+    _one_device(qkv, positions, slots, cos_t, sin_t, q_norm, k_norm, k_cache, v_cache, bias, q_out)
+    with _on(qkv.device):
+        check("le_qk_norm_rope_kv_cache_write", _lib.load().le_qk_norm_rope_kv_cache_write(
+            qkv.data_ptr(), _dt(qkv), _row_stride(qkv),
+            None if bias is None else bias.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), float(eps),
+            positions.data_ptr(), slots.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0], n, q_heads,
+            kv_heads, head_dim, q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _dt(k_cache), num_slots,
+            _stream(stream)))
+    return q_out
+
+
 def argmax_rows(logits: torch.Tensor, stream=None) -> torch.Tensor:
     """First-maximum index of each row of fp32 logits [rows, vocab] (sampler.cpp:9-13)."""
     _req(logits.dtype == torch.float32 and logits.dim() == 2 and logits.is_contiguous() and logits.is_cuda,
@@ -104,6 +182,58 @@ def argmax_rows(logits: torch.Tensor, stream=None) -> torch.Tensor:
     check("le_argmax_rows", _lib.load().le_argmax_rows(_p(logits), logits.shape[0], logits.shape[1], _p(out),
                                                        _stream(stream)))
     return out
+
+
+def verify_drafts_workspace_size(n_seqs: int, n_drafts: int, vocab: int) -> int:
+    return int(_lib.load().le_verify_drafts_workspace_size(n_seqs, n_drafts, vocab))
+
+
+def verify_drafts(logits: torch.Tensor, cu_drafts: torch.Tensor, draft_tokens: torch.Tensor,
+                  accept_u: torch.Tensor, sample_u: torch.Tensor, max_drafts: int,
+                  draft_probs: torch.Tensor | None = None, temperature: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None, n_accepted: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Drafted tokens against the target's logits (le_verify_drafts). logits:
+    [drafts + sequences, vocab], sequence s's rows from cu_drafts[s] + s on;
+    cu_drafts: int32 [sequences + 1]; draft_tokens, accept_u: [drafts];
+    sample_u, temperature: [sequences]; draft_probs: [drafts, vocab], None
+    where the drafts were not sampled. Returns (tokens [sequences,
+    max_drafts + 1] int32: the accepted drafts, the sampled token, then -1;
+    the number accepted [sequences] int32)."""
+    n_drafts, n_seqs = draft_tokens.numel(), cu_drafts.numel() - 1
+    _req(logits.dim() == 2 and logits.is_cuda and logits.stride(1) == 1, "logits: cuda [rows, vocab], unit column stride")
+    _req(n_seqs >= 0 and logits.shape[0] == n_drafts + n_seqs, "logits: one row per draft and one per sequence")
+    vocab = logits.shape[1]
+    _dev_i32(cu_drafts, "cu_drafts")
+    _dev_i32(draft_tokens, "draft_tokens")
+    _dev_f32(accept_u, "accept_u", n_drafts)
+    _dev_f32(sample_u, "sample_u", n_seqs)
+    if temperature is not None:
+        _dev_f32(temperature, "temperature", n_seqs)
+    if draft_probs is not None:
+        _req(draft_probs.is_cuda and draft_probs.shape == (n_drafts, vocab) and draft_probs.stride(1) == 1,
+             "draft_probs: cuda [drafts, vocab], unit column stride")
+    if out is None:
+        out = torch.empty(n_seqs, max_drafts + 1, dtype=torch.int32, device=logits.device)
+    if n_accepted is None:
+        n_accepted = torch.empty(n_seqs, dtype=torch.int32, device=logits.device)
+    _dev_i32(out, "out")
+    _dev_i32(n_accepted, "n_accepted", n_seqs)
+    _req(out.shape == (n_seqs, max_drafts + 1), "out: [sequences, max_drafts + 1]")
+    need = verify_drafts_workspace_size(n_seqs, n_drafts, vocab)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=logits.device)
+    _one_device(logits, cu_drafts, draft_tokens, accept_u, sample_u, temperature, draft_probs, out, n_accepted,
+                workspace)
+    with _on(logits.device):
+        check("le_verify_drafts", _lib.load().le_verify_drafts(
+            logits.data_ptr(), _dt(logits), _row_stride(logits), vocab,
+            None if draft_probs is None else draft_probs.data_ptr(), 0 if draft_probs is None else _dt(draft_probs),
+            0 if draft_probs is None else _row_stride(draft_probs), cu_drafts.data_ptr(), draft_tokens.data_ptr(),
+            accept_u.data_ptr(), sample_u.data_ptr(), None if temperature is None else temperature.data_ptr(), n_seqs,
+            n_drafts, max_drafts, out.data_ptr(), n_accepted.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _stream(stream)))
+    return out, n_accepted
 
 
 def new_workspace(nbytes: int, device="cuda") -> torch.Tensor:
@@ -306,4 +436,85 @@ def ragged_paged_attention_qkv(qkv: torch.Tensor, bias: torch.Tensor | None, cos
         cos_t.shape[0], _p(k_cache), _p(v_cache), _dt(k_cache), num_blocks, ctypes.byref(P), float(scale),
         _p(out), _p(q_scratch), _p(workspace), workspace.numel() * workspace.element_size(),
         _stream(stream)))
+    return out
+
+
+class PrefixPlan:
+    """A step packed for shared_prefix_attention (le_prefix_plan_step): the
+    slices of a Plan; those whose block tables begin with the same ids form
+    groups that read these blocks once. Keeps its pinned host buffer and its
+    device copy."""
+
+    def __init__(self, slices: list[Slice], q_heads: int, kv_heads: int, head_dim: int, block_size: int,
+                 kv_dtype: torch.dtype, partition_tokens: int = 0, device="cuda", pin: bool = True):
+        self.cfg = PlanConfig(q_heads, kv_heads, head_dim, block_size, _dt(kv_dtype), partition_tokens, 0, 0, 0, 0)
+        keep = []
+        arr = (StepSlice * max(1, len(slices)))()
+        for i, s in enumerate(slices):
+            b = np.ascontiguousarray(s.blocks, dtype=np.int32)
+            keep.append(b)
+            arr[i] = StepSlice(s.seq_key, s.start, s.len, int(s.needs_logits), b.size, b.ctypes.data, None)
+        self.plan = PrefixStepPlan()
+        L = _lib.load()
+        st = L.le_prefix_plan_step(arr, len(slices), ctypes.byref(self.cfg), None, 0, ctypes.byref(self.plan))
+        if st != _lib.LE_ENOSPACE:  # (an empty step needs no buffer)
+            check("le_prefix_plan_step", st)
+        nbytes = int(self.plan.bytes)
+        self.host = torch.empty(nbytes, dtype=torch.uint8, pin_memory=pin and torch.cuda.is_available())
+        check("le_prefix_plan_step", L.le_prefix_plan_step(arr, len(slices), ctypes.byref(self.cfg),
+                                                           ctypes.c_void_p(self.host.data_ptr()), nbytes,
+                                                           ctypes.byref(self.plan)))
+        self.device_buf = None
+        self.device = torch.device(device)
+
+    def upload(self, stream=None) -> "PrefixPlan":
+        nbytes = int(self.plan.bytes)
+        if self.device_buf is None or self.device_buf.numel() < nbytes:
+            self.device_buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        with _on(self.device_buf.device):
+            check("le_prefix_plan_upload", _lib.load().le_prefix_plan_upload(
+                ctypes.byref(self.plan), self.host.data_ptr(), self.device_buf.data_ptr(), _stream(stream)))
+        return self
+
+    @property
+    def groups(self) -> int:
+        """Groups of slices that share blocks."""
+        return int(self.plan.n_groups)
+
+    @property
+    def saved_keys(self) -> int:
+        """Cached rows that are not read again (le_prefix_plan.saved_keys)."""
+        return int(self.plan.saved_keys)
+
+    def workspace_size(self) -> int:
+        return int(_lib.load().le_shared_prefix_workspace_size(ctypes.byref(self.plan)))
+
+
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, plan: PrefixPlan,
+                            scale: float, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                            stream=None) -> torch.Tensor:
+    """ragged_paged_attention where sequences share their first blocks
+    (le_shared_prefix_attention): the same result, with the shared keys read
+    once for all rows of a group. q: [N, q_heads*head_dim]; the step's K/V rows
+    are in the caches already."""
+    P = plan.plan
+    cfg = P.cfg
+    _req(plan.device_buf is not None, "plan not uploaded")
+    _req(q.is_cuda and q.is_contiguous() and q.numel() == P.n_tokens * cfg.q_heads * cfg.head_dim,
+         "q: contiguous cuda [N, q_heads*head_dim]")
+    row = cfg.block_size * cfg.kv_heads * cfg.head_dim
+    _req(k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.is_contiguous()
+         and v_cache.is_contiguous() and k_cache.numel() % row == 0, "k/v caches: contiguous, alike, whole blocks")
+    if out is None:
+        out = torch.empty_like(q)
+    _req(out.dtype == q.dtype and out.numel() == q.numel() and out.is_contiguous(), "out like q")
+    need = plan.workspace_size()
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _one_device(q, k_cache, v_cache, plan.device_buf, out, workspace)
+    with _on(q.device):
+        check("le_shared_prefix_attention", _lib.load().le_shared_prefix_attention(
+            q.data_ptr(), _dt(q), k_cache.data_ptr(), v_cache.data_ptr(), _dt(k_cache), k_cache.numel() // row,
+            ctypes.byref(P), float(scale), out.data_ptr(), None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(stream)))
     return out
