@@ -18,6 +18,7 @@ case (drawn from its "lengths" number), values come from the seed.
 """
 from __future__ import annotations
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -34,6 +35,7 @@ MAX_POS = 20480
 EPS = 1e-6
 
 
+@functools.lru_cache(maxsize=1)
 def _kernels():
     if str(ROOT / "llm-engine_amd") not in sys.path:
         sys.path.insert(0, str(ROOT / "llm-engine_amd"))
