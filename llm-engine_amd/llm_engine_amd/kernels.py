@@ -48,41 +48,48 @@ def _dev_i32(t: torch.Tensor, name: str, n: int | None = None) -> None:
         _req(t.numel() >= n, f"{name}: needs {n} entries, has {t.numel()}")
 
 
-def _dev_f32(t: torch.Tensor, name: str, n: int | None = None) -> None:
-    _req(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous(), f"{name}: contiguous fp32 cuda tensor")
-    if n is not None:
-        _req(t.numel() == n, f"{name}: {n} entries, has {t.numel()}")
+# The newer operators are launched from serving loops whose kernels take 3-10 us:
+# their checks are written out (no message is built that is not raised), and the
+# current stream is asked for as a number (2.7 us as a torch.cuda.Stream).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
-    i = first.get_device()
-    for t in others:
-        _req(t is None or t.get_device() == i, "all tensors on one device")
+def _i32(t: torch.Tensor, n: int, device: int) -> bool:
+    return t.get_device() == device and t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= n
+
+
+def _f32(t: torch.Tensor, n: int, device: int) -> bool:
+    return t.get_device() == device and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n
 
 
 def _row_stride(t: torch.Tensor) -> int:
     """Elements from row to row of a 2-d tensor; a single row's is its length
     (whatever its stride says), rounded up to whole 16-byte pieces of any type."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
+    return t.stride(0) if t.size(0) > 1 else (t.size(1) + 7) // 8 * 8
 
 
-class _on:
-    """The tensors' device as the current one for the launch (the current
-    stream is then that device's); costs nothing where it already is."""
+def _bytes(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
 
-    __slots__ = ("want", "was")
 
-    def __init__(self, device: torch.device):
-        self.want = device.index
-
-    def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.want:
-            torch.cuda.set_device(self.want)
-
-    def __exit__(self, *exc):
-        if self.was != self.want:
-            torch.cuda.set_device(self.was)
+def _launch(name: str, device: int, stream, *args) -> None:
+    """Calls an entry point whose last argument is the stream, with the tensors'
+    device as the current one (their stream: that device's current one)."""
+    if stream is None:
+        raw = _raw_stream(device)
+    else:
+        if stream.device.index != device:
+            raise ValueError("stream: of another device than the tensors")
+        raw = stream.cuda_stream
+    fn = getattr(_lib.load(), name)
+    if _current_device() == device:
+        st = fn(*args, raw)
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, raw)
+    if st:
+        check(name, st)
 
 
 def store_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
@@ -142,35 +149,35 @@ def qk_norm_rope_store_kv(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
     rotation: x / sqrt(mean(x^2) + eps) * q_norm or k_norm (fp32 [head_dim]),
     after the bias, in fp32 with one rounding per stored value. Returns q:
     [N, q_heads*head_dim]."""
-    _req(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.is_cuda, "qkv: cuda [N, row] with unit column stride")
-    n, row, kv_dim = qkv.shape[0], (q_heads + 2 * kv_heads) * head_dim, kv_heads * head_dim
-    _req(qkv.shape[1] >= row, "qkv rows too short")
-    _dev_f32(cos_t, "cos_t")
-    _dev_f32(sin_t, "sin_t")
-    _req(cos_t.shape == sin_t.shape and cos_t.dim() == 2 and cos_t.shape[1] == head_dim // 2,
-         "cos/sin: fp32 [max_pos, head_dim/2]")
-    _dev_f32(q_norm, "q_norm", head_dim)
-    _dev_f32(k_norm, "k_norm", head_dim)
-    _req(k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.is_contiguous()
-         and v_cache.is_contiguous() and k_cache.is_cuda and v_cache.is_cuda, "k/v caches must match and be contiguous")
-    num_slots = k_cache.shape[0]
-    _req(k_cache.numel() == num_slots * kv_dim, "cache row size must equal kv_dim")
-    _dev_i32(positions, "positions", n)
-    _dev_i32(slots, "slots", n)
-    if bias is not None:
-        _dev_f32(bias, "bias", row)
+    dev = qkv.get_device()
+    if dev < 0 or qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise ValueError("qkv: cuda [N, row] with unit column stride")
+    n, row, kv_dim, half = qkv.size(0), (q_heads + 2 * kv_heads) * head_dim, kv_heads * head_dim, head_dim // 2
+    if qkv.size(1) < row:
+        raise ValueError("qkv rows too short")
+    max_pos = cos_t.size(0)
+    if cos_t.shape != sin_t.shape or not (_f32(cos_t, max_pos * half, dev) and _f32(sin_t, max_pos * half, dev)):
+        raise ValueError("cos_t, sin_t: contiguous fp32 cuda [max_pos, head_dim/2]")
+    if not (_f32(q_norm, head_dim, dev) and _f32(k_norm, head_dim, dev)):
+        raise ValueError("q_norm, k_norm: contiguous fp32 cuda [head_dim]")
+    num_slots = k_cache.size(0)
+    if not (k_cache.dtype == v_cache.dtype and k_cache.numel() == v_cache.numel() == num_slots * kv_dim
+            and v_cache.size(0) == num_slots and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k_cache.get_device() == v_cache.get_device() == dev):
+        raise ValueError("k_cache, v_cache: contiguous cuda [num_slots, kv_heads*head_dim], alike")
+    if not (_i32(positions, n, dev) and _i32(slots, n, dev)):
+        raise ValueError("positions, slots: contiguous int32 cuda, N entries")
+    if bias is not None and not _f32(bias, row, dev):
+        raise ValueError("bias: contiguous fp32 cuda [q_dim + 2*kv_dim]")
     if q_out is None:
         q_out = torch.empty(n, q_heads * head_dim, dtype=qkv.dtype, device=qkv.device)
-    _req(q_out.is_contiguous() and q_out.dtype == qkv.dtype and q_out.numel() == n * q_heads * head_dim
-         and q_out.is_cuda, "q_out: [N, q_heads*head_dim] in qkv's dtype")
-    _one_device(qkv, positions, slots, cos_t, sin_t, q_norm, k_norm, k_cache, v_cache, bias, q_out)
-    with _on(qkv.device):
-        check("le_qk_norm_rope_kv_cache_write", _lib.load().le_qk_norm_rope_kv_cache_write(
-            qkv.data_ptr(), _dt(qkv), _row_stride(qkv),
-            None if bias is None else bias.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), float(eps),
-            positions.data_ptr(), slots.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0], n, q_heads,
-            kv_heads, head_dim, q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _dt(k_cache), num_slots,
-            _stream(stream)))
+    elif not (q_out.is_contiguous() and q_out.dtype == qkv.dtype and q_out.numel() == n * q_heads * head_dim
+              and q_out.get_device() == dev):
+        raise ValueError("q_out: contiguous cuda [N, q_heads*head_dim] in qkv's dtype")
+    _launch("le_qk_norm_rope_kv_cache_write", dev, stream, qkv.data_ptr(), _dt(qkv), _row_stride(qkv),
+            None if bias is None else bias.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), eps, positions.data_ptr(),
+            slots.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), max_pos, n, q_heads, kv_heads, head_dim,
+            q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _dt(k_cache), num_slots)
     return q_out
 
 
@@ -200,39 +207,42 @@ def verify_drafts(logits: torch.Tensor, cu_drafts: torch.Tensor, draft_tokens: t
     where the drafts were not sampled. Returns (tokens [sequences,
     max_drafts + 1] int32: the accepted drafts, the sampled token, then -1;
     the number accepted [sequences] int32)."""
+    dev = logits.get_device()
     n_drafts, n_seqs = draft_tokens.numel(), cu_drafts.numel() - 1
-    _req(logits.dim() == 2 and logits.is_cuda and logits.stride(1) == 1, "logits: cuda [rows, vocab], unit column stride")
-    _req(n_seqs >= 0 and logits.shape[0] == n_drafts + n_seqs, "logits: one row per draft and one per sequence")
-    vocab = logits.shape[1]
-    _dev_i32(cu_drafts, "cu_drafts")
-    _dev_i32(draft_tokens, "draft_tokens")
-    _dev_f32(accept_u, "accept_u", n_drafts)
-    _dev_f32(sample_u, "sample_u", n_seqs)
-    if temperature is not None:
-        _dev_f32(temperature, "temperature", n_seqs)
-    if draft_probs is not None:
-        _req(draft_probs.is_cuda and draft_probs.shape == (n_drafts, vocab) and draft_probs.stride(1) == 1,
-             "draft_probs: cuda [drafts, vocab], unit column stride")
+    if dev < 0 or logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("logits: cuda [rows, vocab] with unit column stride")
+    vocab = logits.size(1)
+    if n_seqs < 0 or logits.size(0) != n_drafts + n_seqs:
+        raise ValueError("logits: one row per draft and one per sequence")
+    if not (_i32(cu_drafts, n_seqs + 1, dev) and _i32(draft_tokens, n_drafts, dev)):
+        raise ValueError("cu_drafts, draft_tokens: contiguous int32 cuda")
+    if not (_f32(accept_u, n_drafts, dev) and _f32(sample_u, n_seqs, dev)):
+        raise ValueError("accept_u, sample_u: contiguous fp32 cuda, one per draft and one per sequence")
+    if temperature is not None and not _f32(temperature, n_seqs, dev):
+        raise ValueError("temperature: contiguous fp32 cuda, one per sequence")
+    if draft_probs is not None and not (draft_probs.dim() == 2 and draft_probs.size(0) == n_drafts
+                                        and draft_probs.size(1) == vocab and draft_probs.stride(1) == 1
+                                        and draft_probs.get_device() == dev):
+        raise ValueError("draft_probs: cuda [drafts, vocab] with unit column stride")
     if out is None:
         out = torch.empty(n_seqs, max_drafts + 1, dtype=torch.int32, device=logits.device)
+    elif not (_i32(out, 0, dev) and out.dim() == 2 and out.size(0) == n_seqs and out.size(1) == max_drafts + 1):
+        raise ValueError("out: contiguous int32 cuda [sequences, max_drafts + 1]")
     if n_accepted is None:
         n_accepted = torch.empty(n_seqs, dtype=torch.int32, device=logits.device)
-    _dev_i32(out, "out")
-    _dev_i32(n_accepted, "n_accepted", n_seqs)
-    _req(out.shape == (n_seqs, max_drafts + 1), "out: [sequences, max_drafts + 1]")
-    need = verify_drafts_workspace_size(n_seqs, n_drafts, vocab)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=logits.device)
-    _one_device(logits, cu_drafts, draft_tokens, accept_u, sample_u, temperature, draft_probs, out, n_accepted,
-                workspace)
-    with _on(logits.device):
-        check("le_verify_drafts", _lib.load().le_verify_drafts(
-            logits.data_ptr(), _dt(logits), _row_stride(logits), vocab,
+    elif not _i32(n_accepted, n_seqs, dev):
+        raise ValueError("n_accepted: contiguous int32 cuda [sequences]")
+    need = _lib.load().le_verify_drafts_workspace_size(n_seqs, n_drafts, vocab)
+    if _bytes(workspace) < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    elif workspace is not None and workspace.get_device() != dev:
+        raise ValueError("workspace: on the tensors' device")
+    _launch("le_verify_drafts", dev, stream, logits.data_ptr(), _dt(logits), _row_stride(logits), vocab,
             None if draft_probs is None else draft_probs.data_ptr(), 0 if draft_probs is None else _dt(draft_probs),
             0 if draft_probs is None else _row_stride(draft_probs), cu_drafts.data_ptr(), draft_tokens.data_ptr(),
             accept_u.data_ptr(), sample_u.data_ptr(), None if temperature is None else temperature.data_ptr(), n_seqs,
-            n_drafts, max_drafts, out.data_ptr(), n_accepted.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _stream(stream)))
+            n_drafts, max_drafts, out.data_ptr(), n_accepted.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), _bytes(workspace))
     return out, n_accepted
 
 
@@ -464,6 +474,9 @@ class PrefixPlan:
         check("le_prefix_plan_step", L.le_prefix_plan_step(arr, len(slices), ctypes.byref(self.cfg),
                                                            ctypes.c_void_p(self.host.data_ptr()), nbytes,
                                                            ctypes.byref(self.plan)))
+        self._need = int(L.le_shared_prefix_workspace_size(ctypes.byref(self.plan)))
+        self._block = block_size * kv_heads * head_dim
+        self._q_numel = int(self.plan.n_tokens) * q_heads * head_dim
         self.device_buf = None
         self.device = torch.device(device)
 
@@ -471,9 +484,8 @@ class PrefixPlan:
         nbytes = int(self.plan.bytes)
         if self.device_buf is None or self.device_buf.numel() < nbytes:
             self.device_buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        with _on(self.device_buf.device):
-            check("le_prefix_plan_upload", _lib.load().le_prefix_plan_upload(
-                ctypes.byref(self.plan), self.host.data_ptr(), self.device_buf.data_ptr(), _stream(stream)))
+        _launch("le_prefix_plan_upload", self.device_buf.get_device(), stream, ctypes.byref(self.plan),
+                self.host.data_ptr(), self.device_buf.data_ptr())
         return self
 
     @property
@@ -487,7 +499,7 @@ class PrefixPlan:
         return int(self.plan.saved_keys)
 
     def workspace_size(self) -> int:
-        return int(_lib.load().le_shared_prefix_workspace_size(ctypes.byref(self.plan)))
+        return self._need
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, plan: PrefixPlan,
@@ -497,24 +509,25 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     (le_shared_prefix_attention): the same result, with the shared keys read
     once for all rows of a group. q: [N, q_heads*head_dim]; the step's K/V rows
     are in the caches already."""
-    P = plan.plan
-    cfg = P.cfg
-    _req(plan.device_buf is not None, "plan not uploaded")
-    _req(q.is_cuda and q.is_contiguous() and q.numel() == P.n_tokens * cfg.q_heads * cfg.head_dim,
-         "q: contiguous cuda [N, q_heads*head_dim]")
-    row = cfg.block_size * cfg.kv_heads * cfg.head_dim
-    _req(k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype and k_cache.is_contiguous()
-         and v_cache.is_contiguous() and k_cache.numel() % row == 0, "k/v caches: contiguous, alike, whole blocks")
+    dev = q.get_device()
+    if plan.device_buf is None or plan.device_buf.get_device() != dev:
+        raise ValueError("plan not uploaded to the tensors' device")
+    if not q.is_contiguous() or q.numel() != plan._q_numel:
+        raise ValueError("q: contiguous cuda [N, q_heads*head_dim]")
+    blocks, rest = divmod(k_cache.numel(), plan._block)
+    if not (rest == 0 and k_cache.numel() == v_cache.numel() and k_cache.dtype == v_cache.dtype
+            and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and k_cache.get_device() == v_cache.get_device() == dev):
+        raise ValueError("k_cache, v_cache: contiguous cuda, alike, whole blocks")
     if out is None:
         out = torch.empty_like(q)
-    _req(out.dtype == q.dtype and out.numel() == q.numel() and out.is_contiguous(), "out like q")
-    need = plan.workspace_size()
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _one_device(q, k_cache, v_cache, plan.device_buf, out, workspace)
-    with _on(q.device):
-        check("le_shared_prefix_attention", _lib.load().le_shared_prefix_attention(
-            q.data_ptr(), _dt(q), k_cache.data_ptr(), v_cache.data_ptr(), _dt(k_cache), k_cache.numel() // row,
-            ctypes.byref(P), float(scale), out.data_ptr(), None if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(stream)))
+    elif not (out.dtype == q.dtype and out.numel() == q.numel() and out.is_contiguous() and out.get_device() == dev):
+        raise ValueError("out: like q")
+    if _bytes(workspace) < plan._need:
+        workspace = torch.empty(plan._need, dtype=torch.uint8, device=q.device)
+    elif workspace is not None and workspace.get_device() != dev:
+        raise ValueError("workspace: on the tensors' device")
+    _launch("le_shared_prefix_attention", dev, stream, q.data_ptr(), _dt(q), k_cache.data_ptr(), v_cache.data_ptr(),
+            _dt(k_cache), blocks, ctypes.byref(plan.plan), scale, out.data_ptr(),
+            None if workspace is None else workspace.data_ptr(), _bytes(workspace))
     return out
