@@ -12,14 +12,14 @@
 // leave (m, l, o) in fp32 and the merge adds them up:
 //     out = sum_i o_i e^(m_i - M) / sum_i l_i e^(m_i - M),  M = max_i m_i.
 //
-// Four waves load 64 keys at a time into LDS (double buffered, the next
-// tile's loads in registers meanwhile) and share them in one of two ways:
+// Four waves bring 64 keys at a time into LDS (16 each; double buffered, the
+// next tile's loads in registers meanwhile) and share them in one of two ways:
 //   * tiles of more than 32 columns: a wave has 32 columns and all 64 keys
-//     (32x32x16 MFMA);
+//     (32x32x16 MFMA), one barrier a tile;
 //   * up to 32 columns, where three waves would idle: a wave has all columns
-//     and 16 of the 64 keys (16x16 MFMAs), and the four waves' (m, l, o) are
-//     merged at the end. A single row is this case: it is bound by its keys'
-//     bytes, not by the products.
+//     and the 16 keys that it loads itself (16x16 MFMAs, no barrier), and the
+//     four waves' (m, l, o) are merged at the end. A single row is this case:
+//     it is bound by its keys' bytes, not by the products.
 // S^T = K Q^T and O^T = V^T P^T: a lane holds one column, and its scores are
 // the second product's B operand as they are (A and B only have to agree on
 // the order of keys). q enters as it is and the scale is applied to the fp32
@@ -114,33 +114,49 @@ template <> struct mm<float> {
   }
 };
 
-// Rows of the LDS tile, padded: K by 16 bytes (16-byte fragment reads of
-// consecutive rows cover all banks), V by 32 (so do the transposing reads).
-template <typename KV, int HD> struct Tile {
-  static constexpr int KROW = HD * static_cast<int>(sizeof(KV)) + 16;
-  static constexpr int VROW = HD * static_cast<int>(sizeof(KV)) + 32;
-  static constexpr int K_BYTES = kKeys * KROW;
-  static constexpr int BYTES = kKeys * (KROW + VROW);
+// A tile in LDS: 64 K rows, then 64 V rows, no padding (a wave's 16-byte stores
+// fill 1 KB in lane order). Piece s of row r holds the row's piece s ^ f(r), so
+// that neither the 16-byte fragment reads of consecutive rows nor the
+// transposing reads of four rows x 64 bytes meet on a bank.
+template <typename KV, int HD> struct Geo {
+  static constexpr int ES = static_cast<int>(sizeof(KV));
+  static constexpr int ROW = HD * ES;
+  static constexpr int CPR = ROW / 16;         // pieces of a row
+  static constexpr int RPI = kWave / CPR;      // rows that a wave's load covers
+  static constexpr int IPW = 16 / RPI;         // loads of a wave's 16 rows
+  static constexpr int K_BYTES = kKeys * ROW;
+  static constexpr int BYTES = 2 * K_BYTES;
+  __device__ __forceinline__ static int f(int row) {
+    return CPR == 8 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+  }
 };
 template <typename KV, int HD> struct Smem {
-  __attribute__((aligned(16))) char lds[2 * Tile<KV, HD>::BYTES];
+  __attribute__((aligned(16))) char lds[2][Geo<KV, HD>::BYTES];
   float2 ml[kWaves][kNarrow];  // a wave's (max, sum) of each column, at the end
 };
-// the end's accumulators of the four waves, in the tiles' place
+// a row of the end's accumulators, in the tiles' place
 template <int HD> constexpr int kAccRow = HD + 4;
 
-// eight elements of an LDS row as an operand
-template <typename X, typename KV> __device__ __forceinline__ typename mm<X>::frag lds_frag(const char* p) {
-  if constexpr (std::is_same_v<X, float>) {
-    float f[8];
-    elem<KV>::load8(reinterpret_cast<const KV*>(p), f);
+// eight elements from piece `piece` of an LDS row on, as an operand
+template <typename X, typename KV, int HD>
+__device__ __forceinline__ typename mm<X>::frag lds_frag(const char* row, int f, int piece) {
+  const char* p = row + ((piece ^ f) << 4);
+  if constexpr (!std::is_same_v<X, float>) {
+    return mm<X>::load(p);
+  } else {
+    float v[8];
+    elem<KV>::widen(ld16(p), v);
+    if constexpr (sizeof(KV) == 4) elem<KV>::widen(ld16(row + (((piece + 1) ^ f) << 4)), v + 4);
     f32x8 r;
 #pragma unroll
-    for (int e = 0; e < 8; e++) r[e] = f[e];
+    for (int e = 0; e < 8; e++) r[e] = v[e];
     return r;
-  } else {
-    return mm<X>::load(p);
   }
+}
+// one element of an LDS row
+template <typename KV, int HD> __device__ __forceinline__ float lds_elem(const char* row, int f, int i) {
+  constexpr int PE = 16 / static_cast<int>(sizeof(KV));
+  return elem<KV>::load1(reinterpret_cast<const KV*>(row + (((i / PE) ^ f) << 4)) + i % PE);
 }
 
 __device__ __forceinline__ float vmax3(float a, float b, float c) {
@@ -155,6 +171,16 @@ __device__ __forceinline__ float halves_max(float v) {
 __device__ __forceinline__ float halves_sum(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// The last product's result may be read: the compiler counts the wait states of
+// an MFMA result up to its first reader, but not up to one in inline assembly,
+// and not along every way around a conditional block.
+template <typename X> __device__ __forceinline__ void settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (std::is_same_v<X, float>) asm volatile("s_nop 15\n\ts_nop 3");
+  else asm volatile("s_nop 11");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // A query column: its row's token and head, and the last key that it sees,
@@ -194,79 +220,120 @@ __device__ __forceinline__ int64_t record_of(const PrefixParams& p, const Prefix
   return (static_cast<int64_t>(p.part0[c.token]) + it.part) * p.q_heads + c.head;
 }
 
-// Keys of a tile, moved by all threads: a thread has one 16-byte piece of
-// KPT keys' K and V rows.
+// A wave's 16 rows of every tile. The rows' blocks are the wave's (16 keys from
+// a multiple of 16 on lie in one block, or in two of 8), so their addresses are
+// scalars and a lane adds its place in the rows. The block ids of 64 blocks at a
+// time wait in a register, a block a lane.
 template <typename KV, int HD> struct Loader {
-  static constexpr int CPR = HD * static_cast<int>(sizeof(KV)) / 16;
-  static constexpr int KPT = kKeys * CPR / kThreads;
-  static constexpr int KSTEP = kThreads / CPR;
-  using L = Tile<KV, HD>;
+  using L = Geo<KV, HD>;
   const char* kbase;
   const char* vbase;
   const int32_t* ids;
   int64_t row_bytes, num_blocks;
-  int n_keys, key_l, piece, bs_shift, bs_mask;
-  int32_t bid[KPT];
-  uint4 k[KPT], v[KPT];
-  bool ok[KPT];
+  int n_keys, wave, bs_shift, last_blk, window;
+  int32_t id_now, id_next;  // lane i: block 64 * window + i's id, and 64 further
+  uint32_t off[L::IPW];
+  uint4 k[L::IPW], v[L::IPW];  // the tile in flight
+  uint32_t gone;               // bits 0 and 1: its rows 0-7 and 8-15 have no block
 
   __device__ __forceinline__ Loader(const PrefixParams& p, const PrefixItem& it, int kvh) {
-    constexpr int HB = HD * static_cast<int>(sizeof(KV));
-    kbase = static_cast<const char*>(p.k_cache) + static_cast<int64_t>(kvh) * HB;
-    vbase = static_cast<const char*>(p.v_cache) + static_cast<int64_t>(kvh) * HB;
+    const int lane = threadIdx.x & (kWave - 1);
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    kbase = static_cast<const char*>(p.k_cache) + static_cast<int64_t>(kvh) * L::ROW;
+    vbase = static_cast<const char*>(p.v_cache) + static_cast<int64_t>(kvh) * L::ROW;
     ids = p.ids + it.ids_off;
-    row_bytes = static_cast<int64_t>(p.kv_heads) * HB;
+    row_bytes = static_cast<int64_t>(p.kv_heads) * L::ROW;
     num_blocks = p.num_cache_blocks;
     n_keys = it.key_end - it.key_begin;
-    key_l = threadIdx.x / CPR;
-    piece = threadIdx.x - key_l * CPR;
     bs_shift = __builtin_ctz(p.block_size);
-    bs_mask = p.block_size - 1;
-  }
-  __device__ __forceinline__ void fetch_ids(int rel0) {
+    last_blk = (n_keys - 1) >> bs_shift;
+    window = 0;
+    id_now = ids[min(lane, last_blk)];
+    id_next = ids[min(kWave + lane, last_blk)];
 #pragma unroll
-    for (int i = 0; i < KPT; i++) bid[i] = ids[min(rel0 + key_l + i * KSTEP, n_keys - 1) >> bs_shift];
-  }
-  __device__ __forceinline__ void issue(int rel0) {
-#pragma unroll
-    for (int i = 0; i < KPT; i++) {
-      const int rel = rel0 + key_l + i * KSTEP;
-      const bool in = bid[i] >= 0 && bid[i] < num_blocks;
-      ok[i] = in && rel < n_keys;
-      const int64_t off =
-          ((static_cast<int64_t>(in ? bid[i] : 0) << bs_shift) + (min(rel, n_keys - 1) & bs_mask)) * row_bytes + piece * 16;
-      k[i] = ld16(kbase + off);
-      v[i] = ld16(vbase + off);
+    for (int j = 0; j < L::IPW; j++) {
+      const int row = j * L::RPI + lane / L::CPR;
+      off[j] = static_cast<uint32_t>((row & 7) * row_bytes) + (((lane % L::CPR) ^ L::f(row)) << 4);
     }
   }
-  // keys past the range, and blocks outside the cache, become zeros
-  __device__ __forceinline__ void stash(char* b) const {
+  // requests the tile whose first key, relative to the item's, is rel
+  __device__ __forceinline__ void issue(int rel) {
+    const int w = (rel >> bs_shift) >> 6;
+    if (w != window) {
+      window = w;
+      id_now = id_next;
+      id_next = ids[min((w + 1) * kWave + static_cast<int>(threadIdx.x & (kWave - 1)), last_blk)];
+    }
+    gone = 0;
 #pragma unroll
-    for (int i = 0; i < KPT; i++) {
-      const int key = key_l + i * KSTEP;
-      *reinterpret_cast<uint4*>(b + key * L::KROW + piece * 16) = ok[i] ? k[i] : make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(b + L::K_BYTES + key * L::VROW + piece * 16) = ok[i] ? v[i] : make_uint4(0, 0, 0, 0);
+    for (int h = 0; h < 2; h++) {
+      // eight keys (past the range: its last eight again)
+      const int key = min(rel + wave * 16 + h * 8, (n_keys - 1) & ~7);
+      const int id = __builtin_amdgcn_readlane(id_now, (key >> bs_shift) & (kWave - 1));
+      const bool in = id >= 0 && id < num_blocks;
+      gone |= in ? 0u : 1u << h;
+      const int64_t at = ((static_cast<int64_t>(in ? id : 0) << bs_shift) + (key & ((1 << bs_shift) - 1))) * row_bytes;
+#pragma unroll
+      for (int j = h * L::IPW / 2; j < (h + 1) * L::IPW / 2; j++) {
+        k[j] = ld16(kbase + at + off[j]);
+        v[j] = ld16(vbase + at + off[j]);
+      }
+    }
+  }
+  // Puts it into LDS. V rows past the range become zeros (a weight of 0 times
+  // what the cache holds there need not be 0), and K and V rows without a block.
+  __device__ __forceinline__ void stash(char* buf, int rel) const {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int live = n_keys - (rel + wave * 16);
+    char* dst = buf + wave * L::IPW * 1024 + lane * 16;
+#pragma unroll
+    for (int j = 0; j < L::IPW; j++) {
+      *reinterpret_cast<uint4*>(dst + j * 1024) = k[j];
+      *reinterpret_cast<uint4*>(dst + j * 1024 + L::K_BYTES) = v[j];
+    }
+    if (live < 16 || gone != 0) {
+#pragma unroll
+      for (int j = 0; j < L::IPW; j++) {
+        const int row = j * L::RPI + lane / L::CPR;
+        const bool none = (gone >> (row >> 3)) & 1u;
+        if (none) *reinterpret_cast<uint4*>(dst + j * 1024) = make_uint4(0, 0, 0, 0);
+        if (none || row >= live) *reinterpret_cast<uint4*>(dst + j * 1024 + L::K_BYTES) = make_uint4(0, 0, 0, 0);
+      }
     }
   }
 };
+
+// Calls tile(LDS buffer, first key) for the tiles of an item, the first of which
+// is requested already. kShared: the waves read each other's rows.
+template <bool kShared, typename KV, int HD, typename F>
+__device__ __forceinline__ void for_tiles(Loader<KV, HD>& ld, Smem<KV, HD>& sm, F tile) {
+  const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
+  ld.stash(sm.lds[0], 0);
+  for (int t = 0; t < n_tiles; t++) {
+    const int rel = t * kKeys;
+    // all rows of tile t are there, and tile t - 1 is no longer read
+    if constexpr (kShared) __syncthreads();
+    if (t + 1 < n_tiles) ld.issue(rel + kKeys);
+    tile(sm.lds[t & 1], rel);
+    if (t + 1 < n_tiles) ld.stash(sm.lds[(t + 1) & 1], rel + kKeys);
+  }
+}
 
 // ---- more than 32 columns: 32 a wave ----
 template <typename ACT, typename KV, int HD>
 __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixItem& it, int kvh, Smem<KV, HD>& sm) {
   using X = operand<ACT, KV>;
   using M = mm<X>;
-  using L = Tile<KV, HD>;
+  using L = Geo<KV, HD>;
   constexpr int KS = HD / 16, DT = HD / 32, U = kKeys / 32;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const int col = lane & 31, half = lane >> 5, l16 = lane & 15;
   Loader<KV, HD> ld(p, it, kvh);
-  ld.fetch_ids(0);
+  ld.issue(0);
   const Column c = column_of(p, it, kvh, wave * 32 + col);
   typename M::frag qb[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) qb[ks] = q_frag<ACT, X>(p, c, HD, ks * 16 + half * 8);
-  ld.issue(0);
-  ld.fetch_ids(kKeys);
   // the wave's keys: none past the last one that any of its columns sees, and
   // no mask up to the first that one does not (columns without a row aside)
   const int G = p.q_heads / p.kv_heads;
@@ -277,6 +344,8 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
     wave_lim = max(wave_lim, __shfl_xor(wave_lim, d, kWave));
     free_lim = min(free_lim, __shfl_xor(free_lim, d, kWave));
   }
+  wave_lim = __builtin_amdgcn_readfirstlane(any ? wave_lim : -1);
+  free_lim = __builtin_amdgcn_readfirstlane(free_lim);
 
   f32x16 acc[DT];
 #pragma unroll
@@ -285,103 +354,95 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
     for (int e = 0; e < 16; e++) acc[d][e] = 0.f;
   float base = 0.f, thr = -FLT_MAX, lsum = 0.f;  // thr -FLT_MAX: no key yet
   const float scale = p.scale_log2;
-  const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
-  ld.stash(sm.lds);
-  __syncthreads();
-  for (int t = 0; t < n_tiles; t++) {
-    const int rel = t * kKeys;
-    if (t + 1 < n_tiles) {
-      ld.issue(rel + kKeys);
-      ld.fetch_ids(rel + 2 * kKeys);
-    }
-    const char* b = sm.lds + (t & 1) * L::BYTES;
-    if (any && rel <= wave_lim) {
-      f32x16 s[U];
+  for_tiles<true>(ld, sm, [&](const char* b, int rel) {
+    if (rel > wave_lim) return;
+    f32x16 s[U];
+    const int fk = L::f(col);
 #pragma unroll
-      for (int u = 0; u < U; u++) {
+    for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[u][e] = 0.f;
+      for (int e = 0; e < 16; e++) s[u][e] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-          s[u] = M::wide(lds_frag<X, KV>(b + (u * 32 + col) * L::KROW + (ks * 16 + half * 8) * static_cast<int>(sizeof(KV))),
-                         qb[ks], s[u]);
-      }
-      // accumulator e of a lane is key 8 (e / 4) + 4 half + e % 4
-      if (rel + kKeys - 1 > free_lim) {
-        const int m = c.lim - rel - half * 4;
+    for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-          for (int e = 0; e < 16; e++)
-            if (32 * u + 8 * (e / 4) + e % 4 > m) s[u][e] = -INFINITY;
-      }
-      float mt = -INFINITY;
+      for (int u = 0; u < U; u++)
+        s[u] = M::wide(lds_frag<X, KV, HD>(b + (u * 32 + col) * L::ROW, fk, (ks * 16 + half * 8) * L::ES / 16), qb[ks],
+                       s[u]);
+    settle<X>();
+    // accumulator e of a lane is key 8 (e / 4) + 4 half + e % 4
+    if (rel + kKeys - 1 > free_lim) {
+      const int m = c.lim - rel - half * 4;
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) mt = vmax3(mt, s[u][e], s[u][e + 1]);
-      const float y = __builtin_fmaf(mt, scale, -base);
-      if (__builtin_amdgcn_ballot_w64(y > thr)) {
-        // A column's first keys set its base to their maximum; later ones
-        // move it when they pass it by more than kSlack.
-        const float m = halves_max(y);
-        const bool go = m > thr;
-        const float shift = go ? m : 0.f;
-        const float alpha = go && thr != -FLT_MAX ? __builtin_amdgcn_exp2f(-shift) : 1.f;
-        base += shift;
-        thr = go ? kSlack : thr;
-        lsum *= alpha;
+        for (int e = 0; e < 16; e++)
+          if (32 * u + 8 * (e / 4) + e % 4 > m) s[u][e] = -INFINITY;
+    }
+    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int d = 0; d < DT; d++) acc[d] *= alpha;
-      }
+    for (int e = 0; e < 16; e += 4)
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        if constexpr (std::is_same_v<X, float>) {
+      for (int i = 0; i < 4; i++) m4[i] = vmax3(m4[i], s[i >> 1][e + 2 * (i & 1)], s[i >> 1][e + 2 * (i & 1) + 1]);
+    const float mt = vmax2(vmax3(m4[0], m4[1], m4[2]), m4[3]);
+    const float y = __builtin_fmaf(mt, scale, -base);
+    if (__builtin_amdgcn_ballot_w64(y > thr)) {
+      // A column's first keys set its base to their maximum; later ones
+      // move it when they pass it by more than kSlack.
+      const float m = halves_max(y);
+      const bool go = m > thr;
+      const float shift = go ? m : 0.f;
+      const float alpha = go && thr != -FLT_MAX ? __builtin_amdgcn_exp2f(-shift) : 1.f;
+      base += shift;
+      thr = go ? kSlack : thr;
+      lsum *= alpha;
 #pragma unroll
-          for (int e = 0; e < 16; e++) {
-            s[u][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -base));
-            lsum += s[u][e];
-          }
-          const char* vp = b + L::K_BYTES + (u * 32 + 4 * half) * L::VROW + col * static_cast<int>(sizeof(KV));
+      for (int d = 0; d < DT; d++) acc[d] *= alpha;
+    }
 #pragma unroll
-          for (int e = 0; e < 16; e++)
+    for (int u = 0; u < U; u++) {
+      if constexpr (std::is_same_v<X, float>) {
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-              const float a = elem<KV>::load1(reinterpret_cast<const KV*>(
-                  vp + (8 * (e / 4) + e % 4) * L::VROW + d * 32 * static_cast<int>(sizeof(KV))));
-              acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[u][e], acc[d], 0, 0, 0);
-            }
-        } else {
-          typename M::frag pb[2];
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            typename M::pair w;
-            w[0] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -base)));
-            w[1] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e + 1], scale, -base)));
-            pb[e / 8][e % 8] = w[0];
-            pb[e / 8][e % 8 + 1] = w[1];
-            lsum = M::sum2(w, lsum);
-          }
-          // V^T operand of 16 keys: lane (dim 16 (lane / 16 % 2) + lane % 16,
-          // half) holds the keys of accumulators 8 h .. 8 h + 7
-          const char* vp = b + L::K_BYTES + (u * 32 + 4 * half + (l16 >> 2)) * L::VROW + ((lane >> 4) & 1) * 32 + (l16 & 3) * 8;
-#pragma unroll
-          for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-              const auto lo = lds_read_tr16<KV>(vp + 16 * h * L::VROW + d * 64);
-              const auto hi = lds_read_tr16<KV>(vp + (16 * h + 8) * L::VROW + d * 64);
-              const typename M::frag va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-              acc[d] = M::wide(va, pb[h], acc[d]);
-            }
+        for (int e = 0; e < 16; e++) {
+          s[u][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -base));
+          lsum += s[u][e];
         }
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          const int row = 8 * (e / 4) + 4 * half + e % 4;
+#pragma unroll
+          for (int d = 0; d < DT; d++) {
+            const float a = lds_elem<KV, HD>(b + L::K_BYTES + (u * 32 + row) * L::ROW, L::f(row), d * 32 + col);
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[u][e], acc[d], 0, 0, 0);
+          }
+        }
+      } else {
+        typename M::frag pb[2];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          typename M::pair w;
+          w[0] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -base)));
+          w[1] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e + 1], scale, -base)));
+          pb[e / 8][e % 8] = w[0];
+          pb[e / 8][e % 8 + 1] = w[1];
+          lsum = M::sum2(w, lsum);
+        }
+        // V^T operand of 16 keys: lane (dim 16 (lane / 16 % 2) + lane % 16,
+        // half) holds the keys of accumulators 8 h .. 8 h + 7
+        const int row = 4 * half + (l16 >> 2), piece = ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1);
+        const int f_lo = L::f(row), f_hi = L::f(row + 8);
+        const char* vp = b + L::K_BYTES + (u * 32 + row) * L::ROW + (l16 & 1) * 8;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int d = 0; d < DT; d++) {
+            const auto lo = lds_read_tr16<KV>(vp + 16 * h * L::ROW + (((d * 4 + piece) ^ f_lo) << 4));
+            const auto hi = lds_read_tr16<KV>(vp + (16 * h + 8) * L::ROW + (((d * 4 + piece) ^ f_hi) << 4));
+            const typename M::frag va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            acc[d] = M::wide(va, pb[h], acc[d]);
+          }
       }
     }
-    if (t + 1 < n_tiles) {
-      ld.stash(sm.lds + ((t + 1) & 1) * L::BYTES);
-      __syncthreads();
-    }
-  }
+  });
 
   // acc[d][e] = O[column][dim 32 d + 8 (e / 4) + 4 half + e % 4]
   const float l = halves_sum(lsum);
@@ -416,14 +477,14 @@ template <typename ACT, typename KV, int HD, int NC>
 __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixItem& it, int kvh, Smem<KV, HD>& sm) {
   using X = operand<ACT, KV>;
   using M = mm<X>;
-  using L = Tile<KV, HD>;
+  using L = Geo<KV, HD>;
   constexpr int KS = HD / 32, DT = HD / 16;
-  constexpr int ES = static_cast<int>(sizeof(KV));
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & (kWave - 1);
   const int l16 = lane & 15, g = lane >> 4;
   const int G = p.q_heads / p.kv_heads;
   Loader<KV, HD> ld(p, it, kvh);
-  ld.fetch_ids(0);
+  const int wave = ld.wave;
+  ld.issue(0);
   Column c[NC];
   typename M::frag qb[NC][KS];
 #pragma unroll
@@ -432,8 +493,6 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qb[n][ks] = q_frag<ACT, X>(p, c[n], HD, ks * 32 + g * 8);
   }
-  ld.issue(0);
-  ld.fetch_ids(kKeys);
 
   f32x4 acc[NC][DT];
   float m[NC], lsum[NC];
@@ -445,130 +504,124 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
     for (int d = 0; d < DT; d++) acc[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float scale = p.scale_log2;
-  const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
-  ld.stash(sm.lds);
-  __syncthreads();
-  for (int t = 0; t < n_tiles; t++) {
-    const int rel = t * kKeys;
-    if (t + 1 < n_tiles) {
-      ld.issue(rel + kKeys);
-      ld.fetch_ids(rel + 2 * kKeys);
-    }
+  for_tiles<false>(ld, sm, [&](const char* tile, int rel) {
     const int key0 = rel + wave * 16;  // this wave's keys
-    if (key0 < ld.n_keys) {
-      const char* b = sm.lds + (t & 1) * L::BYTES + wave * 16 * L::KROW;
-      const char* bv = sm.lds + (t & 1) * L::BYTES + L::K_BYTES + wave * 16 * L::VROW;
-      f32x4 s[NC];
+    if (key0 >= ld.n_keys) return;
+    const char* b = tile + wave * 16 * L::ROW;
+    const char* bv = b + L::K_BYTES;
+    const int fk = L::f(l16);
+    f32x4 s[NC];
 #pragma unroll
-      for (int n = 0; n < NC; n++) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NC; n++) s[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        const auto ka = lds_frag<X, KV>(b + l16 * L::KROW + (ks * 32 + g * 8) * ES);
+    for (int ks = 0; ks < KS; ks++) {
+      const auto ka = lds_frag<X, KV, HD>(b + l16 * L::ROW, fk, (ks * 32 + g * 8) * L::ES / 16);
 #pragma unroll
-        for (int n = 0; n < NC; n++) s[n] = M::narrow(ka, qb[n][ks], s[n]);
+      for (int n = 0; n < NC; n++) s[n] = M::narrow(ka, qb[n][ks], s[n]);
+    }
+    // accumulator i of a lane is key 4 g + i
+    float w[NC][4];
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+      const int lim = c[n].lim - key0 - 4 * g;
+      float x[4], mt = -FLT_MAX;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        x[i] = i > lim ? -INFINITY : s[n][i] * scale;
+        mt = vmax2(mt, x[i]);
       }
-      // accumulator i of a lane is key 4 g + i
-      float w[NC][4];
+      const float mn = vmax2(m[n], rows_max(mt));
+      if (__builtin_amdgcn_ballot_w64(mn > m[n])) {
+        const float alpha = __builtin_amdgcn_exp2f(m[n] - mn);
+        m[n] = mn;
+        lsum[n] *= alpha;
 #pragma unroll
-      for (int n = 0; n < NC; n++) {
-        const int lim = c[n].lim - key0 - 4 * g;
-        float x[4], mt = -FLT_MAX;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          x[i] = i > lim ? -INFINITY : s[n][i] * scale;
-          mt = vmax2(mt, x[i]);
-        }
-        const float mn = vmax2(m[n], rows_max(mt));
-        if (__builtin_amdgcn_ballot_w64(mn > m[n])) {
-          const float alpha = __builtin_amdgcn_exp2f(m[n] - mn);
-          m[n] = mn;
-          lsum[n] *= alpha;
-#pragma unroll
-          for (int d = 0; d < DT; d++) acc[n][d] *= alpha;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          w[n][i] = __builtin_amdgcn_exp2f(x[i] - m[n]);
-          lsum[n] += w[n][i];
-        }
+        for (int d = 0; d < DT; d++) acc[n][d] *= alpha;
       }
-      if constexpr (std::is_same_v<X, float>) {
-        const char* vp = bv + 4 * g * L::VROW + l16 * ES;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+      for (int i = 0; i < 4; i++) {
+        w[n][i] = __builtin_amdgcn_exp2f(x[i] - m[n]);
+        lsum[n] += w[n][i];
+      }
+    }
+    if constexpr (std::is_same_v<X, float>) {
 #pragma unroll
-          for (int d = 0; d < DT; d++) {
-            const float a = elem<KV>::load1(reinterpret_cast<const KV*>(vp + i * L::VROW + d * 16 * ES));
-#pragma unroll
-            for (int n = 0; n < NC; n++) acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, w[n][i], acc[n][d], 0, 0, 0);
-          }
-      } else {
-        typename mma16<KV>::v4 hi[NC], lo[NC];
-#pragma unroll
-        for (int n = 0; n < NC; n++) {
-  #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            hi[n][i] = static_cast<typename M::scalar>(w[n][i]);
-            lo[n][i] = static_cast<typename M::scalar>(w[n][i] - static_cast<float>(hi[n][i]));
-          }
-        }
-        const char* vp = bv + (4 * g + (l16 >> 2)) * L::VROW + (l16 & 3) * 8;
+      for (int i = 0; i < 4; i++) {
+        const int row = 4 * g + i;
 #pragma unroll
         for (int d = 0; d < DT; d++) {
-          const auto va = lds_read_tr16<KV>(vp + d * 32);
+          const float a = lds_elem<KV, HD>(bv + row * L::ROW, L::f(row), d * 16 + l16);
 #pragma unroll
-          for (int n = 0; n < NC; n++) {
-            acc[n][d] = M::keys16(va, hi[n], acc[n][d]);
-            acc[n][d] = M::keys16(va, lo[n], acc[n][d]);
-          }
+          for (int n = 0; n < NC; n++) acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, w[n][i], acc[n][d], 0, 0, 0);
+        }
+      }
+    } else {
+      typename mma16<KV>::v4 hi[NC], lo[NC];
+#pragma unroll
+      for (int n = 0; n < NC; n++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          hi[n][i] = static_cast<typename M::scalar>(w[n][i]);
+          lo[n][i] = static_cast<typename M::scalar>(w[n][i] - static_cast<float>(hi[n][i]));
+        }
+      }
+      const int row = 4 * g + (l16 >> 2), piece = (l16 & 3) >> 1, f = L::f(row);
+      const char* vp = bv + row * L::ROW + (l16 & 1) * 8;
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const auto va = lds_read_tr16<KV>(vp + (((d * 2 + piece) ^ f) << 4));
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+          acc[n][d] = M::keys16(va, hi[n], acc[n][d]);
+          acc[n][d] = M::keys16(va, lo[n], acc[n][d]);
         }
       }
     }
-    if (t + 1 < n_tiles) {
-      ld.stash(sm.lds + ((t + 1) & 1) * L::BYTES);
-      __syncthreads();
-    }
-  }
+  });
 
-  // ---- the four waves' results, in the tiles' place ----
+  // ---- the four waves' results, in the tiles' place: 16 columns at a time,
+  // waves 0 and 1 in the first buffer, 2 and 3 in the second ----
   // acc[n][d][i] = O[column 16 n + l16][dim 16 d + 4 g + i]
-  constexpr int AR = kAccRow<HD>;
-  static_assert(kWaves * kNarrow * AR * 4 <= 2 * L::BYTES);
-  float* all = reinterpret_cast<float*>(sm.lds);
-  __syncthreads();
+  constexpr int AR = kAccRow<HD>, PIECES = HD / 4;
+  static_assert(2 * 16 * AR * 4 <= L::BYTES);
+  float* mine = reinterpret_cast<float*>(wave < 2 ? sm.lds[0] : sm.lds[1]) + (wave & 1) * 16 * AR;
 #pragma unroll
   for (int n = 0; n < NC; n++) {
     const float l = rows_sum(lsum[n]);
     if (g == 0) sm.ml[wave][n * 16 + l16] = make_float2(m[n], l);
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-      *reinterpret_cast<f32x4*>(all + (wave * kNarrow + n * 16 + l16) * AR + d * 16 + 4 * g) = acc[n][d];
   }
-  __syncthreads();
-  constexpr int PIECES = HD / 4;
-  for (int i = threadIdx.x; i < it.n_rows * G * PIECES; i += kThreads) {
-    const int cc = i / PIECES, d = (i - cc * PIECES) * 4;
-    const Column o = column_of(p, it, kvh, cc);
-    float M4 = -FLT_MAX;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) M4 = fmaxf(M4, sm.ml[w][cc].x);
-    float l = 0.f;
-    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  for (int n = 0; n < NC; n++) {
+    __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-      const float2 x = sm.ml[w][cc];
-      const float f = __builtin_amdgcn_exp2f(x.x - M4);
-      l += x.y * f;
-      a += *reinterpret_cast<const f32x4*>(all + (w * kNarrow + cc) * AR + d) * f;
-    }
-    if (it.part < 0) {
-      const float inv = 1.f / l;
-      const float f[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
-      elem<ACT>::store4(static_cast<ACT*>(p.out) + (static_cast<int64_t>(o.token) * p.q_heads + o.head) * HD + d, f);
-    } else {
-      const int64_t rec = record_of(p, it, o);
-      *reinterpret_cast<f32x4*>(p.acc + rec * HD + d) = a;
-      if (d == 0) p.ml[rec] = make_float2(M4, l);
+    for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4*>(mine + l16 * AR + d * 16 + 4 * g) = acc[n][d];
+    __syncthreads();
+    const int cols = min(16, it.n_rows * G - n * 16);
+    for (int i = threadIdx.x; i < cols * PIECES; i += kThreads) {
+      const int cl = i / PIECES, cc = n * 16 + cl, d = (i - cl * PIECES) * 4;
+      const Column o = column_of(p, it, kvh, cc);
+      float M4 = -FLT_MAX;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) M4 = fmaxf(M4, sm.ml[w][cc].x);
+      float l = 0.f;
+      f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        const float2 x = sm.ml[w][cc];
+        const float f = __builtin_amdgcn_exp2f(x.x - M4);
+        const float* all = reinterpret_cast<const float*>(w < 2 ? sm.lds[0] : sm.lds[1]) + (w & 1) * 16 * AR;
+        l += x.y * f;
+        a += *reinterpret_cast<const f32x4*>(all + cl * AR + d) * f;
+      }
+      if (it.part < 0) {
+        const float inv = 1.f / l;
+        const float f[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
+        elem<ACT>::store4(static_cast<ACT*>(p.out) + (static_cast<int64_t>(o.token) * p.q_heads + o.head) * HD + d, f);
+      } else {
+        const int64_t rec = record_of(p, it, o);
+        *reinterpret_cast<f32x4*>(p.acc + rec * HD + d) = a;
+        if (d == 0) p.ml[rec] = make_float2(M4, l);
+      }
     }
   }
 }
