@@ -314,18 +314,22 @@ typedef struct le_prefix_plan {
   int32_t n_groups;   /* groups of slices that share blocks */
   int32_t n_items;    /* work items (per kv head) */
   int32_t n_parts;    /* partial results of split rows */
+  int32_t rows_stride; /* rows and block ids listed for every item */
+  int32_t ids_stride;
   int32_t reserved_;
   int64_t saved_keys; /* cached rows that are not read again, summed over the groups */
   /* byte offsets inside the packed buffer */
-  int64_t off_items, off_rows, off_ids, off_positions, off_part0, off_row_parts;
+  int64_t off_items, off_rows, off_item_ids, off_ids, off_part0, off_row_parts;
   int64_t bytes;      /* total size of the packed buffer */
   const void* dev;    /* device copy, set by le_prefix_plan_upload */
 } le_prefix_plan;
 
 /* Packs a step for le_shared_prefix_attention: the slices of le_plan_step
  * (`tokens` and `needs_logits` are not read), and of cfg the shape, block size,
- * kv_dtype and partition_tokens (0 = default); flags and table_capacity must be
- * 0. Shared blocks of fewer than 64 keys are not taken together. LE_ENOSPACE
+ * kv_dtype, chunk_q_tile (the most query columns, (row, head) pairs, of a tile:
+ * 32 or 128), partition_tokens and chunk_partition_tokens (keys of a partition
+ * of tiles of at most 32 columns, and of larger ones); 0 = default. flags and
+ * table_capacity must be 0. Shared blocks of fewer than 64 keys are not taken together. LE_ENOSPACE
  * with plan->bytes set if host_cap is too small. */
 int le_prefix_plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* cfg,
                         void* host_buf, int64_t host_cap, le_prefix_plan* plan);

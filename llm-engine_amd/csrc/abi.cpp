@@ -209,7 +209,6 @@ int le_shared_prefix_attention(const void* q, le_dtype act_dtype, const void* k_
   if (cfg.kv_dtype != kv_dtype) return LE_EINVAL;
   if (!plan->dev || !q || !k_cache || !v_cache || !out || !std::isfinite(scale) || num_cache_blocks <= 0)
     return LE_EINVAL;
-  if (cfg.kv_heads > 65535) return LE_EUNSUPPORTED;  // a grid dimension
   if (!aligned16({q, k_cache, v_cache, out})) return LE_EUNSUPPORTED;
   const size_t need = le_shared_prefix_workspace_size(plan);
   if (need > 0 && (!workspace || workspace_bytes < need)) return LE_ENOSPACE;
@@ -219,7 +218,9 @@ int le_shared_prefix_attention(const void* q, le_dtype act_dtype, const void* k_
   le::PrefixParams p{};
   p.q = q; p.k_cache = k_cache; p.v_cache = v_cache; p.out = out;
   p.items = reinterpret_cast<const le::PrefixItem*>(dev + plan->off_items);
-  p.rows = arr(plan->off_rows); p.ids = arr(plan->off_ids); p.positions = arr(plan->off_positions);
+  p.rows = reinterpret_cast<const le::PrefixRow*>(dev + plan->off_rows);
+  p.item_ids = arr(plan->off_item_ids); p.ids = arr(plan->off_ids);
+  p.rows_stride = plan->rows_stride; p.ids_stride = plan->ids_stride;
   p.part0 = arr(plan->off_part0); p.row_parts = arr(plan->off_row_parts);
   if (need > 0) {
     p.acc = static_cast<float*>(workspace);

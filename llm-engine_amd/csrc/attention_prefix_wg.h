@@ -44,7 +44,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kKeys = kPrefixTileKeys;  // keys of an LDS tile
-constexpr int kNarrow = 32;             // columns up to which the waves share keys
+constexpr int kNarrow = kPrefixNarrow;  // columns up to which the waves share keys
 constexpr float kSlack = 8.f;           // log2 units that scores may pass a column's base by
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -133,6 +133,7 @@ template <typename KV, int HD> struct Geo {
 template <typename KV, int HD> struct Smem {
   __attribute__((aligned(16))) char lds[2][Geo<KV, HD>::BYTES];
   float2 ml[kWaves][kNarrow];  // a wave's (max, sum) of each column, at the end
+  int2 row[kNarrow];           // token and first record of each row, for the end
 };
 // a row of the end's accumulators, in the tiles' place
 template <int HD> constexpr int kAccRow = HD + 4;
@@ -183,21 +184,22 @@ template <typename X> __device__ __forceinline__ void settle() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// A query column: its row's token and head, and the last key that it sees,
-// relative to the item's first (negative: none of them).
+// A query column: its row's token and first record, its head, and the last key
+// that it sees, relative to the item's first (negative: none of them).
 struct Column {
-  int token, head, lim;
+  int token, part0, head, lim;
   bool ok;  // the column exists
 };
-__device__ __forceinline__ Column column_of(const PrefixParams& p, const PrefixItem& it, int kvh, int c) {
+__device__ __forceinline__ Column column_of(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int c) {
   const int G = p.q_heads / p.kv_heads;
   const int r = c / G;
+  const PrefixRow row = p.rows[static_cast<int64_t>(item) * p.rows_stride + min(r, p.rows_stride - 1)];
   Column o;
-  const bool ok = r < it.n_rows;
-  o.ok = ok;
-  o.token = p.rows[it.rows_off + (ok ? r : 0)];
-  o.head = kvh * G + (ok ? c - r * G : 0);
-  o.lim = ok ? min(it.key_end - 1, p.positions[o.token]) - it.key_begin : -1;
+  o.ok = r < it.n_rows;
+  o.token = row.token;
+  o.part0 = row.part0;
+  o.head = kvh * G + c - r * G;
+  o.lim = o.ok ? min(it.key_end - 1, row.pos) - it.key_begin : -1;
   return o;
 }
 
@@ -209,21 +211,21 @@ __device__ __forceinline__ typename mm<X>::frag q_frag(const PrefixParams& p, co
   typename mm<X>::frag r;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
-    const float x = c.lim >= 0 ? (p.negate ? -f[e] : f[e]) : 0.f;
+    const float x = c.ok ? (p.negate ? -f[e] : f[e]) : 0.f;
     r[e] = static_cast<typename mm<X>::scalar>(x);
   }
   return r;
 }
 
 // Where a row's part is written: its record's accumulator and (m, l).
-__device__ __forceinline__ int64_t record_of(const PrefixParams& p, const PrefixItem& it, const Column& c) {
-  return (static_cast<int64_t>(p.part0[c.token]) + it.part) * p.q_heads + c.head;
+__device__ __forceinline__ int64_t record_of(const PrefixParams& p, const PrefixItem& it, int part0, int head) {
+  return (static_cast<int64_t>(part0) + it.part) * p.q_heads + head;
 }
 
 // A wave's 16 rows of every tile. The rows' blocks are the wave's (16 keys from
 // a multiple of 16 on lie in one block, or in two of 8), so their addresses are
 // scalars and a lane adds its place in the rows. The block ids of 64 blocks at a
-// time wait in a register, a block a lane.
+// time wait in a register, a block a lane (first_id: the first ones, as listed).
 template <typename KV, int HD> struct Loader {
   using L = Geo<KV, HD>;
   const char* kbase;
@@ -233,10 +235,12 @@ template <typename KV, int HD> struct Loader {
   int n_keys, wave, bs_shift, last_blk, window;
   int32_t id_now, id_next;  // lane i: block 64 * window + i's id, and 64 further
   uint32_t off[L::IPW];
-  uint4 k[L::IPW], v[L::IPW];  // the tile in flight
-  uint32_t gone;               // bits 0 and 1: its rows 0-7 and 8-15 have no block
+  struct Stage {  // a tile in flight
+    uint4 k[L::IPW], v[L::IPW];
+    uint32_t gone;  // bits 0 and 1: its rows 0-7 and 8-15 have no block
+  };
 
-  __device__ __forceinline__ Loader(const PrefixParams& p, const PrefixItem& it, int kvh) {
+  __device__ __forceinline__ Loader(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int32_t first_id) {
     const int lane = threadIdx.x & (kWave - 1);
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     kbase = static_cast<const char*>(p.k_cache) + static_cast<int64_t>(kvh) * L::ROW;
@@ -248,8 +252,8 @@ template <typename KV, int HD> struct Loader {
     bs_shift = __builtin_ctz(p.block_size);
     last_blk = (n_keys - 1) >> bs_shift;
     window = 0;
-    id_now = ids[min(lane, last_blk)];
-    id_next = ids[min(kWave + lane, last_blk)];
+    id_now = first_id;
+    id_next = last_blk >= kWave ? ids[min(kWave + lane, last_blk)] : 0;
 #pragma unroll
     for (int j = 0; j < L::IPW; j++) {
       const int row = j * L::RPI + lane / L::CPR;
@@ -257,45 +261,45 @@ template <typename KV, int HD> struct Loader {
     }
   }
   // requests the tile whose first key, relative to the item's, is rel
-  __device__ __forceinline__ void issue(int rel) {
+  __device__ __forceinline__ void issue(Stage& st, int rel) {
     const int w = (rel >> bs_shift) >> 6;
     if (w != window) {
       window = w;
       id_now = id_next;
       id_next = ids[min((w + 1) * kWave + static_cast<int>(threadIdx.x & (kWave - 1)), last_blk)];
     }
-    gone = 0;
+    st.gone = 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       // eight keys (past the range: its last eight again)
       const int key = min(rel + wave * 16 + h * 8, (n_keys - 1) & ~7);
       const int id = __builtin_amdgcn_readlane(id_now, (key >> bs_shift) & (kWave - 1));
       const bool in = id >= 0 && id < num_blocks;
-      gone |= in ? 0u : 1u << h;
+      st.gone |= in ? 0u : 1u << h;
       const int64_t at = ((static_cast<int64_t>(in ? id : 0) << bs_shift) + (key & ((1 << bs_shift) - 1))) * row_bytes;
 #pragma unroll
       for (int j = h * L::IPW / 2; j < (h + 1) * L::IPW / 2; j++) {
-        k[j] = ld16(kbase + at + off[j]);
-        v[j] = ld16(vbase + at + off[j]);
+        st.k[j] = ld16(kbase + at + off[j]);
+        st.v[j] = ld16(vbase + at + off[j]);
       }
     }
   }
   // Puts it into LDS. V rows past the range become zeros (a weight of 0 times
   // what the cache holds there need not be 0), and K and V rows without a block.
-  __device__ __forceinline__ void stash(char* buf, int rel) const {
+  __device__ __forceinline__ void stash(const Stage& st, char* buf, int rel) const {
     const int lane = threadIdx.x & (kWave - 1);
     const int live = n_keys - (rel + wave * 16);
     char* dst = buf + wave * L::IPW * 1024 + lane * 16;
 #pragma unroll
     for (int j = 0; j < L::IPW; j++) {
-      *reinterpret_cast<uint4*>(dst + j * 1024) = k[j];
-      *reinterpret_cast<uint4*>(dst + j * 1024 + L::K_BYTES) = v[j];
+      *reinterpret_cast<uint4*>(dst + j * 1024) = st.k[j];
+      *reinterpret_cast<uint4*>(dst + j * 1024 + L::K_BYTES) = st.v[j];
     }
-    if (live < 16 || gone != 0) {
+    if (live < 16 || st.gone != 0) {
 #pragma unroll
       for (int j = 0; j < L::IPW; j++) {
         const int row = j * L::RPI + lane / L::CPR;
-        const bool none = (gone >> (row >> 3)) & 1u;
+        const bool none = (st.gone >> (row >> 3)) & 1u;
         if (none) *reinterpret_cast<uint4*>(dst + j * 1024) = make_uint4(0, 0, 0, 0);
         if (none || row >= live) *reinterpret_cast<uint4*>(dst + j * 1024 + L::K_BYTES) = make_uint4(0, 0, 0, 0);
       }
@@ -303,34 +307,56 @@ template <typename KV, int HD> struct Loader {
   }
 };
 
-// Calls tile(LDS buffer, first key) for the tiles of an item, the first of which
-// is requested already. kShared: the waves read each other's rows.
-template <bool kShared, typename KV, int HD, typename F>
-__device__ __forceinline__ void for_tiles(Loader<KV, HD>& ld, Smem<KV, HD>& sm, F tile) {
+// Calls tile(LDS buffer, first key) for the tiles of an item; stage a holds the
+// first one's loads. Shared rows: one tile in flight beside the one in use, and
+// a barrier a tile.
+template <typename KV, int HD, typename F>
+__device__ __forceinline__ void shared_tiles(Loader<KV, HD>& ld, typename Loader<KV, HD>::Stage& a, Smem<KV, HD>& sm,
+                                             F tile) {
   const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
-  ld.stash(sm.lds[0], 0);
+  ld.stash(a, sm.lds[0], 0);
   for (int t = 0; t < n_tiles; t++) {
     const int rel = t * kKeys;
-    // all rows of tile t are there, and tile t - 1 is no longer read
-    if constexpr (kShared) __syncthreads();
-    if (t + 1 < n_tiles) ld.issue(rel + kKeys);
+    __syncthreads();  // all rows of tile t are there, and tile t - 1 is no longer read
+    if (t + 1 < n_tiles) ld.issue(a, rel + kKeys);
     tile(sm.lds[t & 1], rel);
-    if (t + 1 < n_tiles) ld.stash(sm.lds[(t + 1) & 1], rel + kKeys);
+    if (t + 1 < n_tiles) ld.stash(a, sm.lds[(t + 1) & 1], rel + kKeys);
+  }
+}
+// A wave's own rows: two tiles in flight beside the one in use (what bounds
+// such items is how many bytes are on their way), no barrier.
+template <typename KV, int HD, typename F>
+__device__ __forceinline__ void own_tiles(Loader<KV, HD>& ld, typename Loader<KV, HD>::Stage& a, Smem<KV, HD>& sm,
+                                          F tile) {
+  typename Loader<KV, HD>::Stage b;
+  const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
+  if (n_tiles > 1) ld.issue(b, kKeys);
+  for (int t = 0; t < n_tiles; t += 2) {
+    const int rel = t * kKeys;
+    ld.stash(a, sm.lds[0], rel);
+    if (t + 2 < n_tiles) ld.issue(a, rel + 2 * kKeys);
+    tile(sm.lds[0], rel);
+    if (t + 1 >= n_tiles) break;
+    ld.stash(b, sm.lds[1], rel + kKeys);
+    if (t + 3 < n_tiles) ld.issue(b, rel + 3 * kKeys);
+    tile(sm.lds[1], rel + kKeys);
   }
 }
 
 // ---- more than 32 columns: 32 a wave ----
 template <typename ACT, typename KV, int HD>
-__device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixItem& it, int kvh, Smem<KV, HD>& sm) {
+__device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int32_t first_id,
+                                          Smem<KV, HD>& sm) {
   using X = operand<ACT, KV>;
   using M = mm<X>;
   using L = Geo<KV, HD>;
   constexpr int KS = HD / 16, DT = HD / 32, U = kKeys / 32;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const int col = lane & 31, half = lane >> 5, l16 = lane & 15;
-  Loader<KV, HD> ld(p, it, kvh);
-  ld.issue(0);
-  const Column c = column_of(p, it, kvh, wave * 32 + col);
+  Loader<KV, HD> ld(p, it, item, kvh, first_id);
+  typename Loader<KV, HD>::Stage first;
+  ld.issue(first, 0);
+  const Column c = column_of(p, it, item, kvh, wave * 32 + col);
   typename M::frag qb[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) qb[ks] = q_frag<ACT, X>(p, c, HD, ks * 16 + half * 8);
@@ -354,7 +380,7 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
     for (int e = 0; e < 16; e++) acc[d][e] = 0.f;
   float base = 0.f, thr = -FLT_MAX, lsum = 0.f;  // thr -FLT_MAX: no key yet
   const float scale = p.scale_log2;
-  for_tiles<true>(ld, sm, [&](const char* b, int rel) {
+  shared_tiles(ld, first, sm, [&](const char* b, int rel) {
     if (rel > wave_lim) return;
     f32x16 s[U];
     const int fk = L::f(col);
@@ -459,7 +485,7 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
       }
     return;
   }
-  const int64_t rec = record_of(p, it, c);
+  const int64_t rec = record_of(p, it, c.part0, c.head);
   float* o = p.acc + rec * HD + half * 4;
 #pragma unroll
   for (int d = 0; d < DT; d++)
@@ -474,7 +500,8 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
 // tile's products the compiler left the first one's result a wait too short on
 // the way past the branch (fp32: a score without its last product).
 template <typename ACT, typename KV, int HD, int NC>
-__device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixItem& it, int kvh, Smem<KV, HD>& sm) {
+__device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int32_t first_id,
+                                          Smem<KV, HD>& sm) {
   using X = operand<ACT, KV>;
   using M = mm<X>;
   using L = Geo<KV, HD>;
@@ -482,16 +509,22 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
   const int lane = threadIdx.x & (kWave - 1);
   const int l16 = lane & 15, g = lane >> 4;
   const int G = p.q_heads / p.kv_heads;
-  Loader<KV, HD> ld(p, it, kvh);
+  Loader<KV, HD> ld(p, it, item, kvh, first_id);
   const int wave = ld.wave;
-  ld.issue(0);
+  typename Loader<KV, HD>::Stage first;
+  ld.issue(first, 0);
   Column c[NC];
   typename M::frag qb[NC][KS];
 #pragma unroll
   for (int n = 0; n < NC; n++) {
-    c[n] = column_of(p, it, kvh, n * 16 + l16);
+    c[n] = column_of(p, it, item, kvh, n * 16 + l16);
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qb[n][ks] = q_frag<ACT, X>(p, c[n], HD, ks * 32 + g * 8);
+  }
+  if (wave == 0 && g == 0) {
+#pragma unroll
+    for (int n = 0; n < NC; n++)
+      if (c[n].ok) sm.row[(n * 16 + l16) / G] = make_int2(c[n].token, c[n].part0);
   }
 
   f32x4 acc[NC][DT];
@@ -504,7 +537,7 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
     for (int d = 0; d < DT; d++) acc[n][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float scale = p.scale_log2;
-  for_tiles<false>(ld, sm, [&](const char* tile, int rel) {
+  own_tiles(ld, first, sm, [&](const char* tile, int rel) {
     const int key0 = rel + wave * 16;  // this wave's keys
     if (key0 >= ld.n_keys) return;
     const char* b = tile + wave * 16 * L::ROW;
@@ -599,7 +632,8 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
     const int cols = min(16, it.n_rows * G - n * 16);
     for (int i = threadIdx.x; i < cols * PIECES; i += kThreads) {
       const int cl = i / PIECES, cc = n * 16 + cl, d = (i - cl * PIECES) * 4;
-      const Column o = column_of(p, it, kvh, cc);
+      const int row = cc / G, head = kvh * G + cc - row * G;
+      const int2 o = sm.row[row];
       float M4 = -FLT_MAX;
 #pragma unroll
       for (int w = 0; w < kWaves; w++) M4 = fmaxf(M4, sm.ml[w][cc].x);
@@ -616,9 +650,9 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
       if (it.part < 0) {
         const float inv = 1.f / l;
         const float f[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
-        elem<ACT>::store4(static_cast<ACT*>(p.out) + (static_cast<int64_t>(o.token) * p.q_heads + o.head) * HD + d, f);
+        elem<ACT>::store4(static_cast<ACT*>(p.out) + (static_cast<int64_t>(o.x) * p.q_heads + head) * HD + d, f);
       } else {
-        const int64_t rec = record_of(p, it, o);
+        const int64_t rec = record_of(p, it, o.y, head);
         *reinterpret_cast<f32x4*>(p.acc + rec * HD + d) = a;
         if (d == 0) p.ml[rec] = make_float2(M4, l);
       }
@@ -629,12 +663,15 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
 template <typename ACT, typename KV, int HD>
 __global__ __launch_bounds__(kThreads, (std::is_same_v<operand<ACT, KV>, float> ? 1 : 2)) void prefix_kernel(PrefixParams p) {
   __shared__ Smem<KV, HD> sm;
-  const PrefixItem it = p.items[blockIdx.x];
-  const int kvh = blockIdx.y;
+  // an item's kv heads lie side by side: their rows are neighbours in the cache
+  const int item = blockIdx.x / p.kv_heads, kvh = blockIdx.x - item * p.kv_heads;
+  const int32_t first_id = p.item_ids[static_cast<int64_t>(item) * p.ids_stride +
+                                      min(static_cast<int>(threadIdx.x & (kWave - 1)), p.ids_stride - 1)];
+  const PrefixItem it = p.items[item];
   const int cols = it.n_rows * (p.q_heads / p.kv_heads);
-  if (cols <= 16) narrow_item<ACT, KV, HD, 1>(p, it, kvh, sm);
-  else if (cols <= kNarrow) narrow_item<ACT, KV, HD, 2>(p, it, kvh, sm);
-  else wide_item<ACT, KV, HD>(p, it, kvh, sm);
+  if (cols <= 16) narrow_item<ACT, KV, HD, 1>(p, it, item, kvh, first_id, sm);
+  else if (cols <= kNarrow) narrow_item<ACT, KV, HD, 2>(p, it, item, kvh, first_id, sm);
+  else wide_item<ACT, KV, HD>(p, it, item, kvh, first_id, sm);
 }
 
 // ---- rows of several parts: a wave for each (row, head) ----
@@ -693,8 +730,7 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(PrefixParams p) 
 
 template <typename ACT, typename KV, int HD>
 hipError_t launch_prefix(const PrefixParams& p, hipStream_t stream) {
-  prefix_kernel<ACT, KV, HD><<<dim3(static_cast<unsigned>(p.n_items), static_cast<unsigned>(p.kv_heads)), kThreads, 0,
-                               stream>>>(p);
+  prefix_kernel<ACT, KV, HD><<<static_cast<unsigned>(p.n_items) * static_cast<unsigned>(p.kv_heads), kThreads, 0, stream>>>(p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.n_parts == 0) return e;
   const int64_t waves = static_cast<int64_t>(p.n_tokens) * p.q_heads;

@@ -106,29 +106,38 @@ struct VerifyParams {
 size_t verify_workspace(int64_t n_seqs, int64_t n_drafts, int vocab);
 hipError_t verify_drafts(const VerifyParams& p, int logits_dtype, int probs_dtype, void* workspace, hipStream_t stream);
 
-// Shared-prefix attention (attention_prefix_wg.h). A work item: the query rows
-// rows[rows_off .. + n_rows) (token indices) against keys [key_begin, key_end)
-// of the table whose block ids, from key_begin's block on, are at ids_off.
+// Shared-prefix attention (attention_prefix_wg.h). A work item: n_rows query rows
+// against keys [key_begin, key_end) of a block table. Its rows and the ids of
+// its first blocks are listed at the item's index times a stride, so a workgroup
+// requests them without having read the item; the ids of all its blocks, from
+// key_begin's on, are at ids_off too.
 // part: which of its rows' parts this is; -1: their only one, written out.
 // causal: rows see keys up to their own position.
 struct PrefixItem {
-  int32_t rows_off, n_rows, ids_off, key_begin, key_end, part, causal, reserved;
+  int32_t n_rows, ids_off, key_begin, key_end, part, causal, reserved[2];
+};
+// A row of an item: its index in q, its position and its first record.
+struct PrefixRow {
+  int32_t token, pos, part0, reserved;
 };
 constexpr int kPrefixCols = 128;     // query columns (row, head) of an item, at most
+constexpr int kPrefixNarrow = 32;    // columns up to which an item's waves share its keys out
 constexpr int kPrefixTileKeys = 64;  // keys of an LDS tile: partitions are whole tiles
+constexpr int kPrefixListIds = 64;   // block ids listed by item, at most
 struct PrefixParams {
   const void* q;
   const void* k_cache;
   const void* v_cache;
   void* out;
   const PrefixItem* items;
-  const int32_t* rows;
+  const PrefixRow* rows;     // of item i from i * rows_stride on
+  const int32_t* item_ids;   // of item i from i * ids_stride on
   const int32_t* ids;
-  const int32_t* positions;  // of every token
   const int32_t* part0;      // a token's first record; its parts' follow
   const int32_t* row_parts;  // its number of parts
   float* acc;                // [records][q_heads][head_dim] unnormalised
   float2* ml;                // [records][q_heads] (max in log2 units, sum)
+  int rows_stride, ids_stride;
   int n_items, n_tokens, n_parts, q_heads, kv_heads, head_dim, block_size;
   float scale_log2;          // > 0
   int negate;                // the scale was negative: q changes its sign

@@ -24,10 +24,9 @@
 namespace {
 
 using le::PrefixItem;
+using le::PrefixRow;
 
 constexpr int kMinSharedKeys = 64;    // a shorter common beginning is not worth a pass of its own
-constexpr int64_t kTargetWorkgroups = 512;  // two per CU
-constexpr int kMinPart = 128;         // keys of the shortest partition
 constexpr int kMaxParts = 128;        // partitions of a tile
 
 int64_t align256(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
@@ -87,6 +86,14 @@ std::vector<Group> best_groups(const std::vector<int>& lcp, int min_blocks) {
   return groups;
 }
 
+// LDS tiles (64 keys) of a partition, for `work` of them in `count` workgroups.
+int64_t part_tiles(int64_t work, int64_t count, bool narrow) {
+  int64_t t = (work + 255) / 256;
+  if (t > 8) t = std::max<int64_t>(8, (work + 511) / 512);
+  if (narrow && count >= 256) t = std::max<int64_t>(t, 16);
+  return std::max<int64_t>(t, 1);
+}
+
 struct Tile {
   std::vector<int32_t> rows;
   int32_t ids_off;  // block id of key_begin
@@ -103,7 +110,9 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   const int shape = le::check_attention_shape(cfg.q_heads, cfg.kv_heads, cfg.head_dim, cfg.block_size);
   if (shape != LE_OK) return shape;
   if (cfg.kv_dtype != LE_F32 && cfg.kv_dtype != LE_BF16 && cfg.kv_dtype != LE_F16) return LE_EINVAL;
-  if (cfg.partition_tokens < 0 || cfg.flags != 0 || cfg.table_capacity != 0) return LE_EINVAL;
+  if (cfg.partition_tokens < 0 || cfg.chunk_partition_tokens < 0 || cfg.flags != 0 || cfg.table_capacity != 0) return LE_EINVAL;
+  if (cfg.chunk_q_tile != 0 && cfg.chunk_q_tile != le::kPrefixNarrow && cfg.chunk_q_tile != le::kPrefixCols)
+    return LE_EINVAL;
   const int bs = cfg.block_size, G = cfg.q_heads / cfg.kv_heads;
 
   // ---- validation; a key's slices use its first one's table, as le_plan_step's do ----
@@ -150,7 +159,7 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   std::vector<int32_t> ids;
   std::vector<Tile> tiles;
   std::vector<int> shared(n_slices, 0);       // keys of the slice that its group reads
-  const int tile_rows = le::kPrefixCols / G;
+  const int tile_rows = (cfg.chunk_q_tile > 0 ? cfg.chunk_q_tile : le::kPrefixCols) / G;
   auto add_tiles = [&](const std::vector<int32_t>& rows, int32_t ids_off, int begin, bool causal, int end) {
     const int n = static_cast<int>(rows.size());
     const int count = (n + tile_rows - 1) / tile_rows;
@@ -187,54 +196,63 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   if (ids.size() > INT32_MAX / 2) return LE_EUNSUPPORTED;
 
   // ---- partitions ----
-  int64_t work = 0;
-  for (const Tile& t : tiles) work += static_cast<int64_t>(t.key_end - t.key_begin) * cfg.kv_heads;
+  // tiles of more than kPrefixNarrow columns, and the others
   const int quantum = std::max(le::kPrefixTileKeys, bs);
-  int64_t part = cfg.partition_tokens > 0 ? cfg.partition_tokens
-                                          : std::max<int64_t>(kMinPart, work / kTargetWorkgroups);
-  part = (part + quantum - 1) / quantum * quantum;
+  auto wide = [&](const Tile& t) { return static_cast<int>(t.rows.size()) * G > le::kPrefixNarrow; };
+  int64_t work[2] = {0, 0}, count[2] = {0, 0};  // of LDS tiles, and of workgroups if nothing is split
+  for (const Tile& t : tiles) {
+    work[wide(t)] += static_cast<int64_t>(t.key_end - t.key_begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys * cfg.kv_heads;
+    count[wide(t)] += cfg.kv_heads;
+  }
+  int64_t part[2];
+  for (int k = 0; k < 2; k++) {
+    const int asked = k ? cfg.chunk_partition_tokens : cfg.partition_tokens;
+    part[k] = asked > 0 ? asked : part_tiles(work[k], count[k], k == 0) * le::kPrefixTileKeys;
+    part[k] = (part[k] + quantum - 1) / quantum * quantum;
+  }
   std::vector<int32_t> n_parts(static_cast<size_t>(n_tok), 0), part0(static_cast<size_t>(n_tok), 0);
-  int64_t n_items = 0, n_item_rows = 0;
+  int64_t n_items = 0;
   for (Tile& t : tiles) {
     const int64_t units = (t.key_end - t.key_begin + quantum - 1) / quantum;
-    t.parts = static_cast<int>(std::min<int64_t>(kMaxParts, (units * quantum + part - 1) / part));
+    t.parts = static_cast<int>(std::min<int64_t>(kMaxParts, (units * quantum + part[wide(t)] - 1) / part[wide(t)]));
     t.part_first = n_parts[t.rows[0]];
     for (int32_t r : t.rows) n_parts[r] += t.parts;
     n_items += t.parts;
-    n_item_rows += static_cast<int64_t>(t.rows.size());
   }
   int64_t n_records = 0;
   for (int64_t r = 0; r < n_tok; r++) {
     part0[r] = static_cast<int32_t>(n_records);
     if (n_parts[r] > 1) n_records += n_parts[r];
   }
-  if (n_records > INT32_MAX / 2 || n_items > INT32_MAX / 2 || n_item_rows > INT32_MAX / 2) return LE_EUNSUPPORTED;
+  if (n_records > INT32_MAX / 2 || n_items * cfg.kv_heads > INT32_MAX) return LE_EUNSUPPORTED;
 
   // ---- items, longest first ----
-  std::vector<PrefixItem> items;
+  struct Placed {
+    PrefixItem item;
+    const Tile* tile;
+  };
+  std::vector<Placed> items;
   items.reserve(static_cast<size_t>(n_items));
-  std::vector<int32_t> rows;
-  rows.reserve(static_cast<size_t>(n_item_rows));
+  int rows_stride = 1, ids_stride = 1;
   for (const Tile& t : tiles) {
     const int64_t units = (t.key_end - t.key_begin + quantum - 1) / quantum;
-    const int32_t off = static_cast<int32_t>(rows.size());
-    rows.insert(rows.end(), t.rows.begin(), t.rows.end());
     const bool split = n_parts[t.rows[0]] > 1;
+    rows_stride = std::max(rows_stride, static_cast<int>(t.rows.size()));
     for (int k = 0; k < t.parts; k++) {
       PrefixItem it{};
-      it.rows_off = off;
       it.n_rows = static_cast<int32_t>(t.rows.size());
       const int a = static_cast<int>(k * units / t.parts) * quantum, b = static_cast<int>((k + 1) * units / t.parts) * quantum;
       it.key_begin = t.key_begin + a;
-      it.key_end = std::min<int64_t>(static_cast<int64_t>(t.key_begin) + b, t.key_end);
+      it.key_end = static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(t.key_begin) + b, t.key_end));
       it.ids_off = t.ids_off + a / bs;
       it.part = split ? t.part_first + k : -1;
       it.causal = t.causal ? 1 : 0;
-      items.push_back(it);
+      ids_stride = std::max(ids_stride, std::min(le::kPrefixListIds, (it.key_end - it.key_begin + bs - 1) / bs));
+      items.push_back(Placed{it, &t});
     }
   }
-  std::stable_sort(items.begin(), items.end(), [](const PrefixItem& a, const PrefixItem& b) {
-    return a.key_end - a.key_begin > b.key_end - b.key_begin;
+  std::stable_sort(items.begin(), items.end(), [](const Placed& a, const Placed& b) {
+    return a.item.key_end - a.item.key_begin > b.item.key_end - b.item.key_begin;
   });
 
   // ---- layout and copy ----
@@ -251,10 +269,13 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
     off = at;
     at = align256(at + static_cast<int64_t>(bytes));
   };
-  place(out.off_items, items.size() * sizeof(PrefixItem));
-  place(out.off_rows, rows.size() * 4);
+  out.rows_stride = rows_stride;
+  out.ids_stride = ids_stride;
+  const size_t n = items.size();
+  place(out.off_items, n * sizeof(PrefixItem));
+  place(out.off_rows, n * rows_stride * sizeof(PrefixRow));
+  place(out.off_item_ids, n * ids_stride * 4);
   place(out.off_ids, ids.size() * 4);
-  place(out.off_positions, positions.size() * 4);
   place(out.off_part0, part0.size() * 4);
   place(out.off_row_parts, n_parts.size() * 4);
   out.bytes = at;
@@ -262,15 +283,26 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   if (out.bytes == 0) return LE_OK;
   if (!host_buf || host_cap < out.bytes) return LE_ENOSPACE;
   char* dst = static_cast<char*>(host_buf);
-  auto put = [&](int64_t off, const void* src, size_t bytes) {
-    if (bytes) std::memcpy(dst + off, src, bytes);
+  PrefixItem* to_items = reinterpret_cast<PrefixItem*>(dst + out.off_items);
+  PrefixRow* to_rows = reinterpret_cast<PrefixRow*>(dst + out.off_rows);
+  int32_t* to_ids = reinterpret_cast<int32_t*>(dst + out.off_item_ids);
+  for (size_t i = 0; i < n; i++) {
+    const PrefixItem& it = items[i].item;
+    to_items[i] = it;
+    const std::vector<int32_t>& r = items[i].tile->rows;
+    for (int k = 0; k < rows_stride; k++) {
+      const int32_t t = r[std::min<size_t>(k, r.size() - 1)];
+      to_rows[i * rows_stride + k] = PrefixRow{t, positions[t], part0[t], 0};
+    }
+    const int last = (it.key_end - it.key_begin - 1) / bs;
+    for (int k = 0; k < ids_stride; k++) to_ids[i * ids_stride + k] = ids[it.ids_off + std::min(k, last)];
+  }
+  auto put = [&](int64_t off, const std::vector<int32_t>& v) {
+    if (!v.empty()) std::memcpy(dst + off, v.data(), v.size() * 4);
   };
-  put(out.off_items, items.data(), items.size() * sizeof(PrefixItem));
-  put(out.off_rows, rows.data(), rows.size() * 4);
-  put(out.off_ids, ids.data(), ids.size() * 4);
-  put(out.off_positions, positions.data(), positions.size() * 4);
-  put(out.off_part0, part0.data(), part0.size() * 4);
-  put(out.off_row_parts, n_parts.data(), n_parts.size() * 4);
+  put(out.off_ids, ids);
+  put(out.off_part0, part0);
+  put(out.off_row_parts, n_parts);
   return LE_OK;
 }
 

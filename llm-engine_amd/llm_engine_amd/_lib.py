@@ -96,12 +96,14 @@ class PrefixStepPlan(ctypes.Structure):
         ("n_groups", ctypes.c_int32),
         ("n_items", ctypes.c_int32),
         ("n_parts", ctypes.c_int32),
+        ("rows_stride", ctypes.c_int32),
+        ("ids_stride", ctypes.c_int32),
         ("reserved_", ctypes.c_int32),
         ("saved_keys", ctypes.c_int64),
         ("off_items", ctypes.c_int64),
         ("off_rows", ctypes.c_int64),
+        ("off_item_ids", ctypes.c_int64),
         ("off_ids", ctypes.c_int64),
-        ("off_positions", ctypes.c_int64),
         ("off_part0", ctypes.c_int64),
         ("off_row_parts", ctypes.c_int64),
         ("bytes", ctypes.c_int64),

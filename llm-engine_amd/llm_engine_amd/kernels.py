@@ -456,8 +456,10 @@ class PrefixPlan:
     device copy."""
 
     def __init__(self, slices: list[Slice], q_heads: int, kv_heads: int, head_dim: int, block_size: int,
-                 kv_dtype: torch.dtype, partition_tokens: int = 0, device="cuda", pin: bool = True):
-        self.cfg = PlanConfig(q_heads, kv_heads, head_dim, block_size, _dt(kv_dtype), partition_tokens, 0, 0, 0, 0)
+                 kv_dtype: torch.dtype, partition_tokens: int = 0, device="cuda", pin: bool = True,
+                 chunk_q_tile: int = 0, chunk_partition_tokens: int = 0):
+        self.cfg = PlanConfig(q_heads, kv_heads, head_dim, block_size, _dt(kv_dtype), partition_tokens, chunk_q_tile,
+                              chunk_partition_tokens, 0, 0)
         keep = []
         arr = (StepSlice * max(1, len(slices)))()
         for i, s in enumerate(slices):

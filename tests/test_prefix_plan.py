@@ -10,9 +10,6 @@ import torch
 
 from llm_engine_amd import _lib, kernels
 
-ITEM = ("rows_off", "n_rows", "ids_off", "key_begin", "key_end", "part", "causal", "reserved")
-
-
 def pack(seqs, heads=(14, 2, 64), block=16, kv=torch.bfloat16, **kw):
     """seqs: (table, start, rows)."""
     slices = [kernels.Slice(i, a, r, True, np.array(t, dtype=np.int32), np.zeros(a + r, dtype=np.int32))
@@ -27,30 +24,34 @@ def arrays(plan):
         return b[off:off + 4 * n].view(np.int32)
 
     items = at(P.off_items, 8 * P.n_items).reshape(-1, 8)
-    n_rows = int((items[:, 0] + items[:, 1]).max())
-    n_ids = int((P.off_positions - P.off_ids) // 4)
-    return (items, at(P.off_rows, n_rows), at(P.off_ids, n_ids), at(P.off_positions, P.n_tokens),
-            at(P.off_part0, P.n_tokens), at(P.off_row_parts, P.n_tokens))
+    rows = at(P.off_rows, 4 * P.n_items * P.rows_stride).reshape(P.n_items, -1, 4)
+    listed = at(P.off_item_ids, P.n_items * P.ids_stride).reshape(P.n_items, -1)
+    return (items, rows, listed, at(P.off_ids, int((P.off_part0 - P.off_ids) // 4)), at(P.off_part0, P.n_tokens),
+            at(P.off_row_parts, P.n_tokens))
 
 
 def check(seqs, heads=(14, 2, 64), block=16, **kw):
     plan = pack(seqs, heads, block, **kw)
-    items, rows, ids, positions, part0, row_parts = arrays(plan)
+    items, rows, listed, ids, part0, row_parts = arrays(plan)
     G = heads[0] // heads[1]
     tables = [t for t, _, r in seqs for _ in range(r)]
-    assert positions.tolist() == [a + j for _, a, r in seqs for j in range(r)]
+    positions = [a + j for _, a, r in seqs for j in range(r)]
     seen = [np.zeros(p + 1, dtype=int) for p in positions]
     parts = [[] for _ in positions]
-    for off, n, ido, kb, ke, part, causal, _ in items:
+    for i, (n, ido, kb, ke, part, causal, _, _) in enumerate(items):
         assert 0 < n * G <= 128 and 0 <= kb < ke and kb % block == 0
-        for t in rows[off:off + n]:
-            e = min(ke, positions[t] + 1)
-            assert causal or ke <= positions[t] + 1
+        for t, pos, first, _ in rows[i, :n]:
+            assert pos == positions[t] and first == part0[t]
+            e = min(ke, pos + 1)
+            assert causal or ke <= pos + 1
             if e > kb:
                 seen[t][kb:e] += 1
             for b in range(kb // block, (ke - 1) // block + 1):
                 assert ids[ido + b - kb // block] == tables[t][b]
+                if b - kb // block < 64:
+                    assert listed[i, b - kb // block] == tables[t][b]
             parts[t].append(int(part))
+        assert (rows[i, n:, 0] == rows[i, n - 1, 0]).all()  # padded with a row that exists
     assert all((s == 1).all() for s in seen)
     used = 0
     for t, p in enumerate(parts):
@@ -120,7 +121,7 @@ def test_slices_of_one_sequence_use_its_first_table():
     t = np.arange(10, dtype=np.int32)
     s = [kernels.Slice(7, 0, 20, False, t, np.zeros(60, np.int32)), kernels.Slice(7, 20, 4, True, t + 50, np.zeros(60, np.int32))]
     plan = kernels.PrefixPlan(s, 14, 2, 64, 16, torch.bfloat16, device="cpu", pin=False)
-    ids = arrays(plan)[2]
+    ids = arrays(plan)[3]
     assert 50 not in ids and 51 not in ids
 
 
@@ -149,7 +150,8 @@ def test_packer_refusals():
         s = (_lib.StepSlice * 1)(_lib.StepSlice(0, seqs[0][1], seqs[0][2], 1, b.size, b.ctypes.data, None))
         plan = _lib.PrefixStepPlan()
         assert _lib.load().le_prefix_plan_step(s, 1, ctypes.byref(cfg), None, 0, ctypes.byref(plan)) == status, seqs
-    for field, value in (("flags", 4), ("table_capacity", 8), ("kv_dtype", 9), ("partition_tokens", -1)):
+    for field, value in (("flags", 4), ("table_capacity", 8), ("kv_dtype", 9), ("partition_tokens", -1),
+                         ("chunk_q_tile", 16), ("chunk_partition_tokens", -1)):
         cfg = _lib.PlanConfig(14, 2, 64, 16, _lib.LE_BF16, 0, 0, 0, 0, 0)
         setattr(cfg, field, value)
         b = np.arange(4, dtype=np.int32)
