@@ -703,7 +703,8 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(PrefixParams p) 
     const float2 x = ml[static_cast<int64_t>(k0 + min(lane, last)) * p.q_heads];
     const float f = lane <= last ? __builtin_amdgcn_exp2f(x.x - M) : 0.f;
     l += x.y * f;
-    for (int k = group; k <= last; k += 4 * GROUPS) {
+    for (int i = 0; i <= last; i += 4 * GROUPS) {  // (all lanes: a part's factor may be any lane's)
+      const int k = i + group;
       f32x4 v[4];
       float w[4];
 #pragma unroll

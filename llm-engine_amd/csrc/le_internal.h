@@ -83,7 +83,7 @@ struct QkNormParams {
 hipError_t qk_norm_rope_kv_write(const QkNormParams& p, int act_dtype, int cache_dtype, hipStream_t stream);
 
 // Verification of drafted tokens (verify_drafts.hip).
-constexpr int kVerifyPiece = 2048;  // tokens of a row that one wave takes
+constexpr int kVerifyPiece = 8192;  // tokens of a row that one workgroup takes
 struct VerifyParams {
   const void* logits;       // [n_drafts + n_seqs][logits_stride]: sequence s's rows from cu_drafts[s] + s on
   int64_t logits_stride;
@@ -99,9 +99,9 @@ struct VerifyParams {
   int32_t* n_accepted;
   // set by the launcher
   int n_pieces;
-  void* choices;
-  void* stats;
-  double* mass;
+  void* stats;        // of every piece of every target row
+  double* mass;       // [n_seqs][n_pieces]
+  int32_t* arrivals;  // [n_seqs], cleared by the first launch
 };
 size_t verify_workspace(int64_t n_seqs, int64_t n_drafts, int vocab);
 hipError_t verify_drafts(const VerifyParams& p, int logits_dtype, int probs_dtype, void* workspace, hipStream_t stream);

@@ -28,6 +28,8 @@ using le::PrefixRow;
 
 constexpr int kMinSharedKeys = 64;    // a shorter common beginning is not worth a pass of its own
 constexpr int kMaxParts = 128;        // partitions of a tile
+constexpr int kCus = 256;             // MI355X
+constexpr int kSmallF32 = 256;        // LDS tiles of wide fp32 items up to which narrow ones take their place
 
 int64_t align256(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
 
@@ -86,12 +88,23 @@ std::vector<Group> best_groups(const std::vector<int>& lcp, int min_blocks) {
   return groups;
 }
 
-// LDS tiles (64 keys) of a partition, for `work` of them in `count` workgroups.
-int64_t part_tiles(int64_t work, int64_t count, bool narrow) {
-  int64_t t = (work + 255) / 256;
-  if (t > 8) t = std::max<int64_t>(8, (work + 511) / 512);
-  if (narrow && count >= 256) t = std::max<int64_t>(t, 16);
-  return std::max<int64_t>(t, 1);
+// The LDS tiles (64 keys) of a partition: the fewest with which tiles of
+// lengths `len` make at most `slots` workgroups (whole ones where they are more
+// anyway).
+int64_t part_tiles(const std::vector<int64_t>& len, int kv_heads, int64_t slots) {
+  int64_t work = 0, most = 1;
+  for (int64_t n : len) {
+    work += n * kv_heads;
+    most = std::max(most, n);
+  }
+  if (static_cast<int64_t>(len.size()) * kv_heads >= slots) return most;
+  int64_t t = std::max<int64_t>(1, work / slots);
+  for (; t < most; t += std::max<int64_t>(1, t / 16)) {
+    int64_t n = 0;
+    for (int64_t x : len) n += (x + t - 1) / t * kv_heads;
+    if (n <= slots) break;
+  }
+  return std::min(t, most);
 }
 
 struct Tile {
@@ -159,9 +172,16 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   std::vector<int32_t> ids;
   std::vector<Tile> tiles;
   std::vector<int> shared(n_slices, 0);       // keys of the slice that its group reads
-  const int tile_rows = (cfg.chunk_q_tile > 0 ? cfg.chunk_q_tile : le::kPrefixCols) / G;
   auto add_tiles = [&](const std::vector<int32_t>& rows, int32_t ids_off, int begin, bool causal, int end) {
     const int n = static_cast<int>(rows.size());
+    // fp32 products take 3.6 us per 64 keys (head_dim 64) in a wide tile and
+    // 0.9 in a narrow one: a step too small to fill the chip with wide ones is
+    // cut into narrow ones (24 rows behind 1500 keys, 14/2 heads x 64: 12.3 us
+    // against 14.1; 128 rows behind 4096: 42.6 against 34.7).
+    const int64_t wide_tiles = static_cast<int64_t>((n * G + le::kPrefixCols - 1) / le::kPrefixCols) * cfg.kv_heads *
+                               ((end - begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys);
+    const bool small_f32 = cfg.kv_dtype == LE_F32 && wide_tiles <= kSmallF32;
+    const int tile_rows = (cfg.chunk_q_tile > 0 ? cfg.chunk_q_tile : small_f32 ? le::kPrefixNarrow : le::kPrefixCols) / G;
     const int count = (n + tile_rows - 1) / tile_rows;
     for (int k = 0; k < count; k++) {
       const int a = static_cast<int>(static_cast<int64_t>(k) * n / count);
@@ -191,23 +211,41 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
     const int32_t off = static_cast<int32_t>(ids.size());
     const int b0 = shared[i] / bs, b1 = (slices[i].start + slices[i].len - 1) / bs + 1;
     ids.insert(ids.end(), table[i]->blocks + b0, table[i]->blocks + b1);
-    add_tiles(rows, off, shared[i], true, 0);
+    add_tiles(rows, off, shared[i], true, slices[i].start + slices[i].len);
   }
   if (ids.size() > INT32_MAX / 2) return LE_EUNSUPPORTED;
 
   // ---- partitions ----
-  // tiles of more than kPrefixNarrow columns, and the others
+  // Tiles of more than kPrefixNarrow columns are bound by their products and
+  // the chain of a tile's steps, the others by their keys' bytes; a CU holds
+  // two workgroups. So the wide ones are cut to one a CU, beside which the
+  // narrow ones stream (256 rows behind 16384 keys, 32/8 heads x 128, and 64 to
+  // 1024 keys of their own: 178 us, with two a CU 212), or to two where the
+  // narrow ones are few (without own keys: 115 us, with one a CU 120). The
+  // narrow ones are cut to the places left (64 rows behind 4096 keys and 16 to
+  // 512 of their own, 14/2 heads x 64: 14.4 us, cut to two a CU 16.9), with an
+  // fp32 cache, whose products count here too, to one a CU (24 rows behind 1500
+  // keys 12.3 us, two a CU 16.7), but not where they fill the chip as they are,
+  // up to 1024 keys (48 sequences of 5 to 700 keys, 8 kv heads: 19.8 us, cut at
+  // 512 keys 21.9).
   const int quantum = std::max(le::kPrefixTileKeys, bs);
   auto wide = [&](const Tile& t) { return static_cast<int>(t.rows.size()) * G > le::kPrefixNarrow; };
-  int64_t work[2] = {0, 0}, count[2] = {0, 0};  // of LDS tiles, and of workgroups if nothing is split
+  std::vector<int64_t> len[2];
+  int64_t work[2] = {0, 0};
   for (const Tile& t : tiles) {
-    work[wide(t)] += static_cast<int64_t>(t.key_end - t.key_begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys * cfg.kv_heads;
-    count[wide(t)] += cfg.kv_heads;
+    len[wide(t)].push_back((t.key_end - t.key_begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys);
+    work[wide(t)] += len[wide(t)].back();
   }
   int64_t part[2];
+  part[1] = part_tiles(len[1], cfg.kv_heads, work[0] * 8 < work[1] ? 2 * kCus : kCus);
+  int64_t wide_groups = 0;
+  for (int64_t n : len[1]) wide_groups += (n + part[1] - 1) / part[1] * cfg.kv_heads;
+  part[0] = part_tiles(len[0], cfg.kv_heads,
+                       cfg.kv_dtype == LE_F32 ? kCus : 2 * kCus - std::min<int64_t>(wide_groups, kCus));
+  if (static_cast<int64_t>(len[0].size()) * cfg.kv_heads >= kCus) part[0] = std::max<int64_t>(part[0], 16);
   for (int k = 0; k < 2; k++) {
     const int asked = k ? cfg.chunk_partition_tokens : cfg.partition_tokens;
-    part[k] = asked > 0 ? asked : part_tiles(work[k], count[k], k == 0) * le::kPrefixTileKeys;
+    part[k] = asked > 0 ? asked : part[k] * le::kPrefixTileKeys;
     part[k] = (part[k] + quantum - 1) / quantum * quantum;
   }
   std::vector<int32_t> n_parts(static_cast<size_t>(n_tok), 0), part0(static_cast<size_t>(n_tok), 0);

@@ -13,18 +13,24 @@
 // are fp64: a border of the running mass is then off by about 1e-8, where an
 // fp32 sum over 10^5 tokens moves it by 1e-5.
 //
-// A row is read in pieces of kPiece tokens, one wave each, so that one
-// sequence's rows spread over the chip and no barrier is needed: first every
-// target row's (max, sum, first maximum) per piece, then, per sequence, the
-// decision, the rejected row's residual masses per piece, and the token.
+// Two launches. The first reads every target row once, a workgroup a piece of
+// kVerifyPiece tokens, and leaves the piece's (max, sum, first maximum). The
+// second has a workgroup for every (sequence, piece): each forms the decision
+// from the rows' piece statistics (some KB; a launch of its own for it costs
+// more), then the mass of its piece of max(p - q, 0); the last one to arrive
+// picks the token. A row without drafts' probabilities to subtract has its
+// pieces' masses in the statistics already: its first workgroup picks alone.
 #include "le_common.h"
 #include "le_internal.h"
 
 namespace le {
 namespace {
 
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kLaneTokens = 8;                          // consecutive tokens a lane takes at a time
-constexpr int kSteps = kVerifyPiece / (kWave * kLaneTokens);
+constexpr int kWavePiece = kVerifyPiece / kWaves;       // consecutive tokens of a wave
+constexpr int kSteps = kWavePiece / (kWave * kLaneTokens);
+constexpr int kHeldRows = 32;                           // rows whose statistics a workgroup keeps
 
 struct PieceStat {  // 16 bytes
   float m;          // largest logit of the piece (-inf: none)
@@ -32,9 +38,9 @@ struct PieceStat {  // 16 bytes
   double s;         // sum of exp((l - m) / T)
 };
 
-// The row to sample from, as the decision leaves it for the later kernels.
+// The row to sample from.
 struct Choice {
-  int64_t row;      // target row; -1: the sequence's offsets are invalid
+  int64_t row;      // target row
   int64_t q_row;    // its draft row, to be subtracted; -1: none
   int32_t draft;    // the rejected token (drafts without probabilities: its mass is taken out); -1: none
   int32_t column;   // where the token goes
@@ -103,20 +109,22 @@ __device__ __forceinline__ float temperature_of(const VerifyParams& p, int seq) 
 
 // ---- (max, sum, first maximum) of every piece of every target row ----
 template <typename T>
-__global__ __launch_bounds__(256) void stats_kernel(VerifyParams p) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int piece = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int seq = blockIdx.z, j = blockIdx.y;
+__global__ __launch_bounds__(kThreads) void stats_kernel(VerifyParams p) {
+  __shared__ PieceStat part[kWaves];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int piece = blockIdx.x, j = blockIdx.y, seq = blockIdx.z;
+  if (piece == 0 && j == 0 && threadIdx.x == 0) p.arrivals[seq] = 0;
   int begin, n;
-  if (piece >= p.n_pieces || !span_of(p, seq, begin, n) || j > n) return;
+  if (!span_of(p, seq, begin, n) || j > n) return;
   const int64_t row = static_cast<int64_t>(begin) + seq + j;
   const T* l = static_cast<const T*>(p.logits) + row * p.logits_stride;
   const float t = temperature_of(p, seq);
+  const int64_t first = static_cast<int64_t>(piece) * kVerifyPiece + wave * kWavePiece;
   float x[kSteps][kLaneTokens];
   float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kSteps; k++) {
-    const int64_t i = static_cast<int64_t>(piece) * kVerifyPiece + (k * kWave + lane) * kLaneTokens;
+    const int64_t i = first + (k * kWave + lane) * kLaneTokens;
     load_tokens(l, i, p.vocab - i, -INFINITY, x[k]);
   }
 #pragma unroll
@@ -124,26 +132,56 @@ __global__ __launch_bounds__(256) void stats_kernel(VerifyParams p) {
 #pragma unroll
     for (int e = 0; e < kLaneTokens; e++) m = fmaxf(m, x[k][e]);  // NaN is passed over
   m = wave_max(m);
+  float c_hi = 0.f, c_lo = 0.f;
   int arg = INT32_MAX;
-#pragma unroll
-  for (int k = kSteps - 1; k >= 0; k--)
-#pragma unroll
-    for (int e = kLaneTokens - 1; e >= 0; e--)
-      if (x[k][e] == m) arg = piece * kVerifyPiece + (k * kWave + lane) * kLaneTokens + e;
-  arg = wave_min_i32(arg);
   double s = 0.0;
-  if (t > 0.f && m > -INFINITY) {
-    float c_hi, c_lo;
+  if (t > 0.f) {
     factor(t, c_hi, c_lo);
+    if (c_hi > 1e-30f && m < INFINITY) {
+      // the weight without its special cases: what is too far below m to count,
+      // -inf and NaN (a maximum passes over it) come to a weight of 2^-200, 0
+      const float least = -200.f / c_hi;
 #pragma unroll
-    for (int k = 0; k < kSteps; k++)
+      for (int k = 0; k < kSteps; k++) {
+        float w[kLaneTokens];
 #pragma unroll
-      for (int e = 0; e < kLaneTokens; e++) s += weight(x[k][e], m, c_hi, c_lo);
+        for (int e = 0; e < kLaneTokens; e++) {
+          const float d = fmaxf(x[k][e] - m, least);
+          w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(d, c_hi, d * c_lo));
+        }
+        // eight weights in fp32 (three roundings), the rest of the row in fp64
+        s += static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+      }
+      if (!(m > -INFINITY)) s = 0.0;
+    } else {
+#pragma unroll
+      for (int k = 0; k < kSteps; k++)
+#pragma unroll
+        for (int e = 0; e < kLaneTokens; e++) s += m > -INFINITY ? weight(x[k][e], m, c_hi, c_lo) : 0.f;
+    }
     s = wave_sum_f64(s);
+  } else if (m > -INFINITY) {
+#pragma unroll
+    for (int k = kSteps - 1; k >= 0; k--)
+#pragma unroll
+      for (int e = kLaneTokens - 1; e >= 0; e--)
+        if (x[k][e] == m) arg = static_cast<int>(first) + (k * kWave + lane) * kLaneTokens + e;
+    arg = wave_min_i32(arg);
   }
-  if (lane == 0) {
-    PieceStat* st = static_cast<PieceStat*>(p.stats) + row * p.n_pieces + piece;
-    *st = PieceStat{m, m > -INFINITY ? arg : -1, s};
+  if (lane == 0) part[wave] = PieceStat{m, arg, s};
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    PieceStat all = part[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) all.m = fmaxf(all.m, part[w].m);
+    all.arg = INT32_MAX;
+    all.s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+      if (part[w].m == all.m) all.arg = min(all.arg, part[w].arg);
+      if (part[w].m > -INFINITY) all.s += part[w].s * static_cast<double>(weight(part[w].m, all.m, c_hi, c_lo));
+    }
+    static_cast<PieceStat*>(p.stats)[row * p.n_pieces + piece] = all;
   }
 }
 
@@ -156,17 +194,22 @@ struct RowStat {
 __device__ __forceinline__ RowStat row_stat(const VerifyParams& p, int64_t row, float c_hi, float c_lo) {
   const int lane = threadIdx.x & (kWave - 1);
   const PieceStat* st = static_cast<const PieceStat*>(p.stats) + row * p.n_pieces;
-  float m = -INFINITY;
-  for (int i = lane; i < p.n_pieces; i += kWave) m = fmaxf(m, st[i].m);
-  m = wave_max(m);
-  int arg = INT32_MAX;
-  double s = 0.0;
+  PieceStat own{-INFINITY, INT32_MAX, 0.0};  // of this lane's pieces
   for (int i = lane; i < p.n_pieces; i += kWave) {
     const PieceStat a = st[i];
-    if (a.m == m && a.arg >= 0) arg = min(arg, a.arg);
-    s += a.s * static_cast<double>(weight(a.m, m, c_hi, c_lo));
+    if (!(a.m > -INFINITY)) continue;
+    if (a.m > own.m) {
+      own.s = a.s + (own.m > -INFINITY ? own.s * static_cast<double>(weight(own.m, a.m, c_hi, c_lo)) : 0.0);
+      own.m = a.m;
+      own.arg = a.arg;
+    } else {
+      own.s += a.s * static_cast<double>(weight(a.m, own.m, c_hi, c_lo));
+      if (a.m == own.m) own.arg = min(own.arg, a.arg);
+    }
   }
-  return RowStat{m, wave_min_i32(arg), wave_sum_f64(s)};
+  const float m = wave_max(own.m);
+  const double s = own.m > -INFINITY ? own.s * static_cast<double>(weight(own.m, m, c_hi, c_lo)) : 0.0;
+  return RowStat{m, wave_min_i32(own.m == m ? own.arg : INT32_MAX), wave_sum_f64(s)};
 }
 
 // exp((l - m) / T) in fp64, for the one token that is compared with a random number
@@ -174,73 +217,6 @@ __device__ __forceinline__ double weight_f64(float l, float m, float t) {
   if (l == m) return 1.0;
   if (!(l < m) || l == -INFINITY || m == INFINITY) return 0.0;
   return exp((static_cast<double>(l) - static_cast<double>(m)) / static_cast<double>(t));
-}
-
-// ---- a sequence's accepted drafts, and the row its next token comes from ----
-template <typename T, typename Q>
-__global__ __launch_bounds__(256) void decide_kernel(VerifyParams p) {
-  __shared__ int first;  // the first row that is not accepted
-  const int seq = blockIdx.x;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  Choice* choice = static_cast<Choice*>(p.choices) + seq;
-  int32_t* out = p.out + static_cast<int64_t>(seq) * (p.max_drafts + 1);
-  for (int i = threadIdx.x; i <= p.max_drafts; i += 256) out[i] = -1;
-  int begin, n;
-  if (!span_of(p, seq, begin, n)) {
-    if (threadIdx.x == 0) {
-      p.n_accepted[seq] = -1;
-      choice->row = -1;
-    }
-    return;
-  }
-  if (threadIdx.x == 0) first = n;
-  __syncthreads();
-  const float t = temperature_of(p, seq);
-  float c_hi = 0.f, c_lo = 0.f;
-  if (t > 0.f) factor(t, c_hi, c_lo);
-  const T* logits = static_cast<const T*>(p.logits);
-  const Q* probs = static_cast<const Q*>(p.draft_probs);
-  for (int j = wave; j < n; j += 4) {
-    const int64_t row = static_cast<int64_t>(begin) + seq + j;
-    const RowStat r = row_stat(p, row, c_hi, c_lo);
-    if (lane == 0) {
-      const int x = p.draft_tokens[begin + j];
-      bool ok = false;
-      if (x >= 0 && x < p.vocab) {
-        const double q = probs ? static_cast<double>(elem<Q>::load1(probs + (begin + j) * p.probs_stride + x)) : 1.0;
-        const double u = static_cast<double>(p.accept_u[begin + j]);
-        double w, s = 1.0;
-        if (t > 0.f && r.m > -INFINITY) {
-          w = weight_f64(elem<T>::load1(logits + row * p.logits_stride + x), r.m, t);
-          s = r.s;
-        } else {
-          w = x == (r.m > -INFINITY ? r.arg : 0) ? 1.0 : 0.0;
-        }
-        ok = u * q * s < w;
-      }
-      if (!ok) atomicMin(&first, j);
-    }
-  }
-  __syncthreads();
-  const int acc = first;
-  for (int j = threadIdx.x; j < acc; j += 256) out[j] = p.draft_tokens[begin + j];
-  if (wave != 0) return;
-  const int64_t row = static_cast<int64_t>(begin) + seq + acc;
-  const RowStat r = row_stat(p, row, c_hi, c_lo);
-  if (lane == 0) {
-    p.n_accepted[seq] = acc;
-    Choice c;
-    c.row = row;
-    c.q_row = acc < n && probs ? begin + acc : -1;
-    c.draft = acc < n && !probs ? p.draft_tokens[begin + acc] : -1;
-    c.column = acc;
-    c.m = r.m;
-    c.c_hi = c_hi;
-    c.c_lo = c_lo;
-    c.only = !(r.m > -INFINITY) ? 0 : (t > 0.f ? -1 : r.arg);
-    c.inv_s = 1.0 / r.s;
-    *choice = c;
-  }
 }
 
 // The masses of a lane's eight tokens from i on; residual: less the draft's.
@@ -259,28 +235,6 @@ __device__ __forceinline__ void masses(const VerifyParams& p, const Choice& c, i
   }
 }
 
-// ---- masses of every piece of the row to sample from ----
-template <typename T, typename Q>
-__global__ __launch_bounds__(256) void mass_kernel(VerifyParams p) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int piece = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int seq = blockIdx.y;
-  if (piece >= p.n_pieces) return;
-  const Choice c = static_cast<const Choice*>(p.choices)[seq];
-  if (c.row < 0 || c.only >= 0) return;
-  double s = 0.0;
-#pragma unroll
-  for (int k = 0; k < kSteps; k++) {
-    const int64_t i = static_cast<int64_t>(piece) * kVerifyPiece + (k * kWave + lane) * kLaneTokens;
-    double w[kLaneTokens];
-    masses<T, Q>(p, c, i, true, w);
-#pragma unroll
-    for (int e = 0; e < kLaneTokens; e++) s += w[e];
-  }
-  s = wave_sum_f64(s);
-  if (lane == 0) p.mass[static_cast<int64_t>(seq) * p.n_pieces + piece] = s;
-}
-
 __device__ __forceinline__ double wave_scan_f64(double v) {  // inclusive
   const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
@@ -291,94 +245,244 @@ __device__ __forceinline__ double wave_scan_f64(double v) {  // inclusive
   return v;
 }
 
-// ---- the token: the piece that the border falls into, then the place in it ----
+// ---- the decision, the masses of the row to sample from, and the token ----
+struct VerifySmem {
+  RowStat rows[kHeldRows];
+  Choice choice;
+  int first;             // the first row that is not accepted
+  int last;              // this workgroup arrived last
+  double sum[kWaves];
+  double border, before;  // random number times the whole mass; mass before the piece
+  int piece, residual, token, tail;
+};
+
+// A sequence's accepted drafts, and the row its next token comes from: left in
+// sm.choice. Every workgroup of the sequence comes to the same result; `writes`
+// one of them writes it out.
 template <typename T, typename Q>
-__global__ __launch_bounds__(kWave) void pick_kernel(VerifyParams p) {
-  const int lane = threadIdx.x, seq = blockIdx.x;
-  const Choice c = static_cast<const Choice*>(p.choices)[seq];
-  if (c.row < 0) return;
-  int32_t* out = p.out + static_cast<int64_t>(seq) * (p.max_drafts + 1) + c.column;
-  if (c.only >= 0) {
-    if (lane == 0) *out = c.only;
-    return;
-  }
-  const double u = static_cast<double>(p.sample_u[seq]);
-  const double* mass = p.mass + static_cast<int64_t>(seq) * p.n_pieces;
-  const PieceStat* st = static_cast<const PieceStat*>(p.stats) + c.row * p.n_pieces;
-  bool residual = true;
-  auto piece_mass = [&](int i) {
-    if (i >= p.n_pieces) return 0.0;
-    return residual ? mass[i] : st[i].s * static_cast<double>(weight(st[i].m, c.m, c.c_hi, c.c_lo)) * c.inv_s;
-  };
-  auto total_of = [&]() {
-    double s = 0.0;
-    for (int i = lane; i < p.n_pieces; i += kWave) s += piece_mass(i);
-    return wave_sum_f64(s);
-  };
-  double total = total_of();
-  if (!(total > 0.0)) {
-    residual = false;
-    total = total_of();
-  }
-  const double border = u * total;
-  // the first piece whose running mass exceeds the border; the last one with
-  // any mass where none does (u of 1 or more, NaN, or the sums' last bits)
-  int piece = -1, last = -1;
-  double before = 0.0, run = 0.0, last_before = 0.0;
-  for (int i0 = 0; i0 < p.n_pieces && piece < 0; i0 += kWave) {
-    const double w = piece_mass(i0 + lane);
-    const double sum = run + wave_scan_f64(w);
-    const uint64_t over = __builtin_amdgcn_ballot_w64(w > 0.0 && sum > border);
-    const uint64_t any = __builtin_amdgcn_ballot_w64(w > 0.0);
-    if (over) {
-      const int at = __builtin_ctzll(over);
-      piece = i0 + at;
-      before = __shfl(sum, at, kWave) - __shfl(w, at, kWave);
-    } else if (any) {
-      const int at = 63 - __builtin_clzll(any);
-      last = i0 + at;
-      last_before = __shfl(sum, at, kWave) - __shfl(w, at, kWave);
-    }
-    run = __shfl(sum, kWave - 1, kWave);
-  }
-  if (piece < 0) {
-    piece = last;
-    before = last_before;
-  }
-  int token = -1, tail = 0;  // tail: the last token of the piece with any mass
-  run = before;
-  for (int k = 0; k < kSteps && piece >= 0 && token < 0; k++) {
-    const int64_t i = static_cast<int64_t>(piece) * kVerifyPiece + (k * kWave + lane) * kLaneTokens;
-    double w[kLaneTokens], own = 0.0;
-    masses<T, Q>(p, c, i, residual, w);
-#pragma unroll
-    for (int e = 0; e < kLaneTokens; e++) own += w[e];
-    const double upto = run + wave_scan_f64(own);
-    double at = upto - own;
-    int mine = INT32_MAX, final_mine = -1;
-#pragma unroll
-    for (int e = 0; e < kLaneTokens; e++) {
-      at += w[e];
-      if (w[e] > 0.0) {
-        if (at > border) mine = min(mine, static_cast<int>(i) + e);
-        final_mine = static_cast<int>(i) + e;
+__device__ __forceinline__ void decide(const VerifyParams& p, VerifySmem& sm, int seq, int begin, int n, bool writes) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  if (threadIdx.x == 0) sm.first = n;
+  __syncthreads();
+  const float t = temperature_of(p, seq);
+  float c_hi = 0.f, c_lo = 0.f;
+  if (t > 0.f) factor(t, c_hi, c_lo);
+  const T* logits = static_cast<const T*>(p.logits);
+  const Q* probs = static_cast<const Q*>(p.draft_probs);
+  for (int j = wave; j <= n; j += kWaves) {
+    const int64_t row = static_cast<int64_t>(begin) + seq + j;
+    // the draft's own values, on their way beside the statistics
+    int x = -1;
+    float u = 0.f, l = 0.f, q = 1.f;
+    if (j < n) {
+      x = p.draft_tokens[begin + j];
+      u = p.accept_u[begin + j];
+      if (x >= 0 && x < p.vocab) {
+        l = elem<T>::load1(logits + row * p.logits_stride + x);
+        if (probs) q = elem<Q>::load1(probs + (static_cast<int64_t>(begin) + j) * p.probs_stride + x);
       }
     }
-    const int got = wave_min_i32(mine);
-    if (got != INT32_MAX) token = got;
-    const int fin = -wave_min_i32(-final_mine);
-    if (fin >= 0) tail = fin;
+    const RowStat r = row_stat(p, row, c_hi, c_lo);
+    if (lane == 0) {
+      if (j < kHeldRows) sm.rows[j] = r;
+      if (j < n) {
+        bool ok = false;
+        if (x >= 0 && x < p.vocab) {
+          double w, s = 1.0;
+          if (t > 0.f && r.m > -INFINITY) {
+            w = weight_f64(l, r.m, t);
+            s = r.s;
+          } else {
+            w = x == (r.m > -INFINITY ? r.arg : 0) ? 1.0 : 0.0;
+          }
+          ok = static_cast<double>(u) * static_cast<double>(q) * s < w;
+        }
+        if (!ok) atomicMin(&sm.first, j);
+      }
+    }
+  }
+  __syncthreads();
+  const int acc = sm.first;
+  if (wave == 0) {
+    const int64_t row = static_cast<int64_t>(begin) + seq + acc;
+    const RowStat r = acc < kHeldRows ? sm.rows[acc] : row_stat(p, row, c_hi, c_lo);
+    if (lane == 0) {
+      Choice c;
+      c.row = row;
+      c.q_row = acc < n && probs ? static_cast<int64_t>(begin) + acc : -1;
+      c.draft = acc < n && !probs ? p.draft_tokens[begin + acc] : -1;
+      c.column = acc;
+      c.m = r.m;
+      c.c_hi = c_hi;
+      c.c_lo = c_lo;
+      c.only = !(r.m > -INFINITY) ? 0 : (t > 0.f ? -1 : r.arg);
+      c.inv_s = 1.0 / r.s;
+      sm.choice = c;
+    }
+  }
+  if (writes) {
+    int32_t* out = p.out + static_cast<int64_t>(seq) * (p.max_drafts + 1);
+    for (int i = threadIdx.x; i <= p.max_drafts; i += kThreads)
+      if (i != acc) out[i] = i < acc ? p.draft_tokens[begin + i] : -1;
+    if (threadIdx.x == 0) p.n_accepted[seq] = acc;
+  }
+  __syncthreads();
+}
+
+// The token: the piece that the border falls into, then the place in it.
+template <typename T, typename Q>
+__device__ __forceinline__ int pick(const VerifyParams& p, VerifySmem& sm, int seq) {
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const Choice c = sm.choice;
+  if (wave == 0) {
+    double* mass = p.mass + static_cast<int64_t>(seq) * p.n_pieces;
+    const PieceStat* st = static_cast<const PieceStat*>(p.stats) + c.row * p.n_pieces;
+    // written by this launch's workgroups where something is subtracted (read past this XCD's L2)
+    bool residual = c.q_row >= 0 || c.draft >= 0;
+    auto piece_mass = [&](int i) {
+      if (i >= p.n_pieces) return 0.0;
+      if (residual) return __hip_atomic_load(mass + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const PieceStat a = st[i];
+      return a.m > -INFINITY ? a.s * static_cast<double>(weight(a.m, c.m, c.c_hi, c.c_lo)) * c.inv_s : 0.0;
+    };
+    auto total_of = [&]() {
+      double s = 0.0;
+      for (int i = lane; i < p.n_pieces; i += kWave) s += piece_mass(i);
+      return wave_sum_f64(s);
+    };
+    double total = total_of();
+    if (residual && !(total > 0.0)) {
+      residual = false;
+      total = total_of();
+    }
+    const double border = static_cast<double>(p.sample_u[seq]) * total;
+    // the first piece whose running mass exceeds the border; the last one with
+    // any mass where none does (u of 1 or more, NaN, or the sums' last bits)
+    int piece = -1, last = -1;
+    double before = 0.0, run = 0.0, last_before = 0.0;
+    for (int i0 = 0; i0 < p.n_pieces && piece < 0; i0 += kWave) {
+      const double w = piece_mass(i0 + lane);
+      const double sum = run + wave_scan_f64(w);
+      const uint64_t over = __builtin_amdgcn_ballot_w64(w > 0.0 && sum > border);
+      const uint64_t any = __builtin_amdgcn_ballot_w64(w > 0.0);
+      if (over) {
+        const int at = __builtin_ctzll(over);
+        piece = i0 + at;
+        before = __shfl(sum, at, kWave) - __shfl(w, at, kWave);
+      } else if (any) {
+        const int at = 63 - __builtin_clzll(any);
+        last = i0 + at;
+        last_before = __shfl(sum, at, kWave) - __shfl(w, at, kWave);
+      }
+      run = __shfl(sum, kWave - 1, kWave);
+    }
+    if (lane == 0) {
+      sm.piece = piece >= 0 ? piece : max(last, 0);
+      sm.before = piece >= 0 ? before : last_before;
+      sm.border = border;
+      sm.residual = residual;
+      sm.token = INT32_MAX;
+      sm.tail = 0;
+    }
+  }
+  __syncthreads();
+  const bool residual = sm.residual != 0;
+  const double border = sm.border;
+  const int64_t first = static_cast<int64_t>(sm.piece) * kVerifyPiece + wave * kWavePiece;
+  double w[kSteps][kLaneTokens], own[kSteps], all = 0.0;
+#pragma unroll
+  for (int k = 0; k < kSteps; k++) {
+    masses<T, Q>(p, c, first + (k * kWave + lane) * kLaneTokens, residual, w[k]);
+    own[k] = 0.0;
+#pragma unroll
+    for (int e = 0; e < kLaneTokens; e++) own[k] += w[k][e];
+    all += own[k];
+  }
+  all = wave_sum_f64(all);
+  if (lane == 0) sm.sum[wave] = all;
+  __syncthreads();
+  double run = sm.before;
+  for (int i = 0; i < wave; i++) run += sm.sum[i];
+  int mine = INT32_MAX, tail = -1;
+#pragma unroll
+  for (int k = 0; k < kSteps; k++) {
+    const double upto = run + wave_scan_f64(own[k]);
+    double at = upto - own[k];
+    const int i = static_cast<int>(first) + (k * kWave + lane) * kLaneTokens;
+#pragma unroll
+    for (int e = 0; e < kLaneTokens; e++) {
+      at += w[k][e];
+      if (w[k][e] > 0.0) {
+        if (at > border) mine = min(mine, i + e);
+        tail = i + e;
+      }
+    }
     run = __shfl(upto, kWave - 1, kWave);
   }
-  if (lane == 0) *out = token >= 0 ? token : tail;
+  if (mine != INT32_MAX) atomicMin(&sm.token, mine);
+  if (tail >= 0) atomicMax(&sm.tail, tail);  // the last token of the piece with any mass
+  __syncthreads();
+  return sm.token != INT32_MAX ? sm.token : sm.tail;
+}
+
+template <typename T, typename Q>
+__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyParams p) {
+  __shared__ VerifySmem sm;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const int piece = blockIdx.x, seq = blockIdx.y;
+  int32_t* out = p.out + static_cast<int64_t>(seq) * (p.max_drafts + 1);
+  int begin, n;
+  if (!span_of(p, seq, begin, n)) {
+    if (piece == 0) {
+      for (int i = threadIdx.x; i <= p.max_drafts; i += kThreads) out[i] = -1;
+      if (threadIdx.x == 0) p.n_accepted[seq] = -1;
+    }
+    return;
+  }
+  if (piece > 0 && (n == 0 || !(temperature_of(p, seq) > 0.f))) return;  // nothing to subtract
+  decide<T, Q>(p, sm, seq, begin, n, piece == 0);
+  const Choice& c = sm.choice;
+  if (c.only >= 0) {
+    if (piece == 0 && threadIdx.x == 0) out[c.column] = c.only;
+    return;
+  }
+  if (c.q_row < 0 && c.draft < 0) {
+    if (piece > 0) return;
+  } else {
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < kSteps; k++) {
+      double w[kLaneTokens];
+      masses<T, Q>(p, c, static_cast<int64_t>(piece) * kVerifyPiece + wave * kWavePiece + (k * kWave + lane) * kLaneTokens,
+                   true, w);
+#pragma unroll
+      for (int e = 0; e < kLaneTokens; e++) s += w[e];
+    }
+    s = wave_sum_f64(s);
+    if (lane == 0) sm.sum[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double all = 0.0;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) all += sm.sum[w];
+      __hip_atomic_store(p.mass + static_cast<int64_t>(seq) * p.n_pieces + piece, all, __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+      __builtin_amdgcn_s_waitcnt(0);  // the mass is where every XCD reads it before the arrival counts
+      sm.last = __hip_atomic_fetch_add(p.arrivals + seq, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.n_pieces - 1;
+    }
+    __syncthreads();
+    if (!sm.last) return;
+  }
+  const int token = pick<T, Q>(p, sm, seq);
+  if (threadIdx.x == 0) out[c.column] = token;
 }
 
 }  // namespace
 
 size_t verify_workspace(int64_t n_seqs, int64_t n_drafts, int vocab) {
   const size_t pieces = (static_cast<size_t>(vocab) + kVerifyPiece - 1) / kVerifyPiece;
-  return static_cast<size_t>(n_seqs) * sizeof(Choice) + static_cast<size_t>(n_seqs + n_drafts) * pieces * sizeof(PieceStat) +
-         static_cast<size_t>(n_seqs) * pieces * sizeof(double);
+  return static_cast<size_t>(n_seqs + n_drafts) * pieces * sizeof(PieceStat) +
+         static_cast<size_t>(n_seqs) * (pieces * sizeof(double) + sizeof(int32_t));
 }
 
 hipError_t verify_drafts(const VerifyParams& in, int logits_dtype, int probs_dtype, void* workspace,
@@ -386,20 +490,19 @@ hipError_t verify_drafts(const VerifyParams& in, int logits_dtype, int probs_dty
   VerifyParams p = in;
   p.n_pieces = (p.vocab - 1) / kVerifyPiece + 1;
   char* ws = static_cast<char*>(workspace);
-  p.choices = ws;
-  ws += static_cast<size_t>(p.n_seqs) * sizeof(Choice);
   p.stats = ws;
   ws += static_cast<size_t>(p.n_seqs + p.n_drafts) * p.n_pieces * sizeof(PieceStat);
   p.mass = reinterpret_cast<double*>(ws);
-  const unsigned groups = static_cast<unsigned>((p.n_pieces + 3) / 4), seqs = static_cast<unsigned>(p.n_seqs);
+  p.arrivals = reinterpret_cast<int32_t*>(ws + static_cast<size_t>(p.n_seqs) * p.n_pieces * sizeof(double));
+  const unsigned pieces = static_cast<unsigned>(p.n_pieces), seqs = static_cast<unsigned>(p.n_seqs);
   return with_dtype(logits_dtype, [&](auto a) {
     return with_dtype(probs_dtype, [&](auto b) {
       using T = decltype(a);
       using Q = decltype(b);
-      stats_kernel<T><<<dim3(groups, static_cast<unsigned>(p.max_drafts + 1), seqs), 256, 0, stream>>>(p);
-      decide_kernel<T, Q><<<seqs, 256, 0, stream>>>(p);
-      mass_kernel<T, Q><<<dim3(groups, seqs), 256, 0, stream>>>(p);
-      pick_kernel<T, Q><<<seqs, kWave, 0, stream>>>(p);
+      stats_kernel<T><<<dim3(pieces, static_cast<unsigned>(p.max_drafts + 1), seqs), kThreads, 0, stream>>>(p);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      verify_kernel<T, Q><<<dim3(pieces, seqs), kThreads, 0, stream>>>(p);
       return hipGetLastError();
     });
   });

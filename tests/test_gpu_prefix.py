@@ -179,6 +179,13 @@ def test_partitions_agree(gpu, part):
     Step(seqs, QWEN, seed=10, partition_tokens=part).check()
 
 
+@pytest.mark.parametrize("heads", [QWEN, WIDE])
+def test_numbers_of_parts(gpu, heads):
+    """Rows of 2 to 129 parts, one more or less than what a wave takes at a time."""
+    own = [64 * n - 3 for n in (1, 2, 3, 6, 7, 8, 9, 14, 15, 16, 17, 30, 31, 32, 33, 47, 62, 63, 64, 65, 100, 128)]
+    Step([(0, 8, k, 1) for k in own], heads, seed=20, partition_tokens=64, chunk_partition_tokens=128).check()
+
+
 @pytest.mark.parametrize("kv", ["bf16", "f16", "f32"])
 def test_dead_cache_rows_are_not_read(gpu, kv):
     """NaN in every cache row that no sequence has computed (the rest of the last
