@@ -7,30 +7,45 @@
 //     drafts, row d from p_d: the first token whose running mass exceeds
 //     u * (whole mass); where max(p - q, 0) is nothing, from p.
 //
-// A token's weight is e = exp2((l - m) log2(e) / T) in fp32, at most 1; the
-// factor is kept in two terms, since its rounding would shift every weight of
-// a row alike. Sums of weights and everything compared with a random number
-// are fp64: a border of the running mass is then off by about 1e-8, where an
-// fp32 sum over 10^5 tokens moves it by 1e-5.
+// A token's weight is e = exp2((l - m) log2(e) / T) in fp32, at most 1, and its
+// mass max(e / S - q, 0), fp32 too; the factors log2(e) / T and 1 / S are kept in
+// two terms each, since their rounding would shift every weight of a row alike.
+// Sums (past eight tokens) and everything compared with a random number are
+// fp64: a border of the running mass is then off by about 1e-8, where an fp32
+// sum over 10^5 tokens moves it by 1e-5. (fp64 masses, which the weights' own
+// roundings do not merit: 64 sequences x 151936 tokens 4 us slower.)
 //
 // Two launches. The first reads every target row once, a workgroup a piece of
 // kVerifyPiece tokens, and leaves the piece's (max, sum, first maximum). The
-// second has a workgroup for every (sequence, piece): each forms the decision
-// from the rows' piece statistics (some KB; a launch of its own for it costs
-// more), then the mass of its piece of max(p - q, 0); the last one to arrive
-// picks the token. A row without drafts' probabilities to subtract has its
+// second has several workgroups for a sequence, about two a CU in all: each
+// forms the decision from the rows' piece statistics (some KB; a launch of its
+// own for it costs more), then the masses of its pieces of max(p - q, 0); the
+// last one to arrive picks the token. A row without drafts' probabilities to subtract has its
 // pieces' masses in the statistics already: its first workgroup picks alone.
+//
+// The second launch is a chain of short steps, each run once: what bounds it is
+// how many memory round trips and cross-lane reductions follow each other, and
+// fetching its instructions. So a workgroup has 16 waves, a row's statistics or
+// 512 of the piece's tokens each, reductions are register moves (DPP) instead of
+// LDS ones, and loops are not unrolled (four waves, shuffles and 25 KB of code
+// took 18 us for one sequence, without the copies of code 14; now 9). A workgroup
+// a piece, 1216 of them, took 30 us for 64 sequences x 151936 tokens.
+#include <algorithm>
+#include <type_traits>
+
 #include "le_common.h"
 #include "le_internal.h"
 
 namespace le {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kLaneTokens = 8;                          // consecutive tokens a lane takes at a time
-constexpr int kWavePiece = kVerifyPiece / kWaves;       // consecutive tokens of a wave
-constexpr int kSteps = kWavePiece / (kWave * kLaneTokens);
-constexpr int kHeldRows = 32;                           // rows whose statistics a workgroup keeps
+constexpr int kLaneTokens = 8;                     // consecutive tokens a lane takes at a time
+constexpr int kStepTokens = kWave * kLaneTokens;   // and a wave
+constexpr int kThreads = 256, kWaves = kThreads / kWave;  // the first launch
+constexpr int kSteps = kVerifyPiece / (kWaves * kStepTokens);
+constexpr int kPickWaves = kVerifyPiece / kStepTokens, kPickThreads = kPickWaves * kWave;  // the second
+static_assert(kPickWaves == 16);
+constexpr int kOwnPieces = 32;                     // pieces of one workgroup there, at most
 
 struct PieceStat {  // 16 bytes
   float m;          // largest logit of the piece (-inf: none)
@@ -46,24 +61,33 @@ struct Choice {
   int32_t column;   // where the token goes
   float m, c_hi, c_lo;
   int32_t only;     // >= 0: the token is this one (T <= 0, or no logit above -inf)
-  double inv_s;     // 1 / sum of the row's weights
+  float s_hi, s_lo; // 1 / sum of the row's weights
 };
 
-// Eight consecutive elements at i, of which n are in the row; the others come
-// back as `fill`. Rows need no more than their element's alignment: the
-// vector loads say so (memory takes them at any address).
+// A lane's eight tokens from i on, and `skip`: the first of them that are not its
+// own. Past the row's end the last eight tokens are read again and skipped, so
+// there is one way to read a row; rows of fewer than eight tokens (TINY) are
+// read one by one. Rows need no more than their element's alignment: the vector
+// loads say so (memory takes them at any address).
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Eight { T v[8]; };
-template <typename T>
-__device__ __forceinline__ void load_tokens(const T* row, int64_t i, int64_t n, float fill, float* o) {
-  if (n >= kLaneTokens) {
-    const Eight<T> r = *reinterpret_cast<const Eight<T>*>(row + i);
-#pragma unroll
-    for (int e = 0; e < kLaneTokens; e++) o[e] = elem<T>::load1(&r.v[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < kLaneTokens; e++) o[e] = e < n ? elem<T>::load1(row + i + e) : fill;
+template <bool TINY> struct Place {
+  int first, skip;  // token of the first element, elements of another lane
+  __device__ __forceinline__ Place(int i, int vocab) {
+    first = TINY ? 0 : min(i, vocab - kLaneTokens);
+    skip = i - first;
   }
-}
+  template <typename T> __device__ __forceinline__ void load(const T* row, int vocab, float* o) const {
+    if constexpr (TINY) {
+#pragma unroll
+      for (int e = 0; e < kLaneTokens; e++) o[e] = elem<T>::load1(row + min(e, vocab - 1));
+    } else {
+      const Eight<T> r = *reinterpret_cast<const Eight<T>*>(row + first);
+#pragma unroll
+      for (int e = 0; e < kLaneTokens; e++) o[e] = elem<T>::load1(&r.v[e]);
+    }
+  }
+  __device__ __forceinline__ bool has(int e, int vocab) const { return e >= skip && (!TINY || e < vocab); }
+};
 
 // weight of a logit under the row's maximum m > -inf; NaN and -inf weigh
 // nothing (nor does a finite logit under +inf, or one too far below m: a
@@ -84,15 +108,60 @@ __device__ __forceinline__ void factor(float t, float& c_hi, float& c_lo) {
   }
 }
 
+// Eight weights in fp32 (three roundings), to be added up in fp64.
+__device__ __forceinline__ double sum8(const float* w) {
+  return static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+}
+
+// Cross-lane moves of 64-bit values; a lane that CTRL gives no source gets 0.
+template <int CTRL> __device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double f64_of(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// Sum over the wave, the same in every lane.
 __device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) v += __shfl_xor(v, d, kWave);
-  return v;
+  v += dpp_f64<dpp::kXor1>(v);
+  v += dpp_f64<dpp::kXor2>(v);
+  v += dpp_f64<dpp::kHalfMirror>(v);
+  v += dpp_f64<dpp::kMirror>(v);
+  uint64_t u = __builtin_bit_cast(uint64_t, v);
+  auto lo = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+  u = __builtin_bit_cast(uint64_t, f64_of(lo[0], hi[0]) + f64_of(lo[1], hi[1]));
+  lo = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(u), static_cast<uint32_t>(u), false, false);
+  hi = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(u >> 32), static_cast<uint32_t>(u >> 32), false, false);
+  return f64_of(lo[0], hi[0]) + f64_of(lo[1], hi[1]);
+}
+// Inclusive sums over the lanes: within the rows of 16, then with the totals
+// of the rows before.
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return f64_of(__builtin_amdgcn_readlane(static_cast<int>(u), lane), __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane));
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
+  v += dpp_f64<0x111>(v);  // row_shr:1
+  v += dpp_f64<0x112>(v);
+  v += dpp_f64<0x114>(v);
+  v += dpp_f64<0x118>(v);
+  const int row = (threadIdx.x & (kWave - 1)) >> 4;
+  const double r0 = lane_f64(v, 15), r1 = r0 + lane_f64(v, 31), r2 = r1 + lane_f64(v, 47);
+  return row == 0 ? v : v + (row == 1 ? r0 : row == 2 ? r1 : r2);
+}
+template <int CTRL> __device__ __forceinline__ int dpp_i32(int v) {
+  return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false);
 }
 __device__ __forceinline__ int wave_min_i32(int v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) v = min(v, __shfl_xor(v, d, kWave));
-  return v;
+  v = min(v, dpp_i32<dpp::kXor1>(v));
+  v = min(v, dpp_i32<dpp::kXor2>(v));
+  v = min(v, dpp_i32<dpp::kHalfMirror>(v));
+  v = min(v, dpp_i32<dpp::kMirror>(v));
+  return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
 // A sequence's drafts [begin, begin + n); false where its offsets are not
@@ -108,7 +177,7 @@ __device__ __forceinline__ float temperature_of(const VerifyParams& p, int seq) 
 }
 
 // ---- (max, sum, first maximum) of every piece of every target row ----
-template <typename T>
+template <typename T, bool TINY>
 __global__ __launch_bounds__(kThreads) void stats_kernel(VerifyParams p) {
   __shared__ PieceStat part[kWaves];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
@@ -119,13 +188,18 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(VerifyParams p) {
   const int64_t row = static_cast<int64_t>(begin) + seq + j;
   const T* l = static_cast<const T*>(p.logits) + row * p.logits_stride;
   const float t = temperature_of(p, seq);
-  const int64_t first = static_cast<int64_t>(piece) * kVerifyPiece + wave * kWavePiece;
+  const int first = piece * kVerifyPiece + wave * kSteps * kStepTokens;
+  auto place = [&](int k) { return Place<TINY>(first + k * kStepTokens + lane * kLaneTokens, p.vocab); };
   float x[kSteps][kLaneTokens];
   float m = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < kSteps; k++) {
-    const int64_t i = first + (k * kWave + lane) * kLaneTokens;
-    load_tokens(l, i, p.vocab - i, -INFINITY, x[k]);
+  for (int k = 0; k < kSteps; k++) place(k).load(l, p.vocab, x[k]);
+  if (first + kSteps * kStepTokens > p.vocab) {  // what another lane has too, or nobody
+#pragma unroll
+    for (int k = 0; k < kSteps; k++)
+#pragma unroll
+      for (int e = 0; e < kLaneTokens; e++)
+        if (!place(k).has(e, p.vocab)) x[k][e] = -INFINITY;
   }
 #pragma unroll
   for (int k = 0; k < kSteps; k++)
@@ -149,34 +223,37 @@ __global__ __launch_bounds__(kThreads) void stats_kernel(VerifyParams p) {
           const float d = fmaxf(x[k][e] - m, least);
           w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(d, c_hi, d * c_lo));
         }
-        // eight weights in fp32 (three roundings), the rest of the row in fp64
-        s += static_cast<double>(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+        s += sum8(w);
       }
       if (!(m > -INFINITY)) s = 0.0;
-    } else {
+    } else if (m > -INFINITY) {
+#pragma unroll 1
+      for (int k = 0; k < kSteps; k++) {
+        const Place<TINY> at = place(k);
+        float y[kLaneTokens];
+        at.load(l, p.vocab, y);
 #pragma unroll
-      for (int k = 0; k < kSteps; k++)
-#pragma unroll
-        for (int e = 0; e < kLaneTokens; e++) s += m > -INFINITY ? weight(x[k][e], m, c_hi, c_lo) : 0.f;
+        for (int e = 0; e < kLaneTokens; e++) s += at.has(e, p.vocab) ? weight(y[e], m, c_hi, c_lo) : 0.f;
+      }
     }
     s = wave_sum_f64(s);
   } else if (m > -INFINITY) {
-#pragma unroll
-    for (int k = kSteps - 1; k >= 0; k--)
+#pragma unroll 1
+    for (int k = kSteps - 1; k >= 0; k--) {
+      const Place<TINY> at = place(k);
+      float y[kLaneTokens];
+      at.load(l, p.vocab, y);
 #pragma unroll
       for (int e = kLaneTokens - 1; e >= 0; e--)
-        if (x[k][e] == m) arg = static_cast<int>(first) + (k * kWave + lane) * kLaneTokens + e;
+        if (at.has(e, p.vocab) && y[e] == m) arg = at.first + e;
+    }
     arg = wave_min_i32(arg);
   }
   if (lane == 0) part[wave] = PieceStat{m, arg, s};
   __syncthreads();
   if (threadIdx.x == 0) {
-    PieceStat all = part[0];
-#pragma unroll
+    PieceStat all{part[0].m, INT32_MAX, 0.0};
     for (int w = 1; w < kWaves; w++) all.m = fmaxf(all.m, part[w].m);
-    all.arg = INT32_MAX;
-    all.s = 0.0;
-#pragma unroll
     for (int w = 0; w < kWaves; w++) {
       if (part[w].m == all.m) all.arg = min(all.arg, part[w].arg);
       if (part[w].m > -INFINITY) all.s += part[w].s * static_cast<double>(weight(part[w].m, all.m, c_hi, c_lo));
@@ -219,60 +296,52 @@ __device__ __forceinline__ double weight_f64(float l, float m, float t) {
   return exp((static_cast<double>(l) - static_cast<double>(m)) / static_cast<double>(t));
 }
 
-// The masses of a lane's eight tokens from i on; residual: less the draft's.
-template <typename T, typename Q>
-__device__ __forceinline__ void masses(const VerifyParams& p, const Choice& c, int64_t i, bool residual, double* w) {
+// The masses of a lane's eight tokens; residual: less the draft's.
+template <typename T, typename Q, bool TINY>
+__device__ __forceinline__ void masses(const VerifyParams& p, const Choice& c, const Place<TINY>& at, bool residual,
+                                       float* w) {
   float l[kLaneTokens], q[kLaneTokens];
-  load_tokens(static_cast<const T*>(p.logits) + c.row * p.logits_stride, i, p.vocab - i, -INFINITY, l);
+  at.load(static_cast<const T*>(p.logits) + c.row * p.logits_stride, p.vocab, l);
   const bool less = residual && c.q_row >= 0;
-  if (less)
-    load_tokens(static_cast<const Q*>(p.draft_probs) + c.q_row * p.probs_stride, i, p.vocab - i, 0.f, q);
+#pragma unroll
+  for (int e = 0; e < kLaneTokens; e++) q[e] = 0.f;
+  if (less) at.load(static_cast<const Q*>(p.draft_probs) + c.q_row * p.probs_stride, p.vocab, q);
 #pragma unroll
   for (int e = 0; e < kLaneTokens; e++) {
-    w[e] = static_cast<double>(weight(l[e], c.m, c.c_hi, c.c_lo)) * c.inv_s;
-    if (less) w[e] = fmax(w[e] - static_cast<double>(q[e]), 0.0);  // a NaN leaves nothing
-    if (residual && i + e == c.draft) w[e] = 0.0;
+    const float x = weight(l[e], c.m, c.c_hi, c.c_lo);
+    const float left = fmaxf(__builtin_fmaf(x, c.s_hi, __builtin_fmaf(x, c.s_lo, -q[e])), 0.f);  // (of a NaN: nothing)
+    w[e] = at.has(e, p.vocab) && !(residual && at.first + e == c.draft) ? left : 0.f;
   }
 }
-
-__device__ __forceinline__ double wave_scan_f64(double v) {  // inclusive
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const double o = __shfl_up(v, d, kWave);
-    if (lane >= d) v += o;
-  }
-  return v;
-}
-
 // ---- the decision, the masses of the row to sample from, and the token ----
 struct VerifySmem {
-  RowStat rows[kHeldRows];
   Choice choice;
-  int first;             // the first row that is not accepted
-  int last;              // this workgroup arrived last
-  double sum[kWaves];
+  int first;              // the first row that is not accepted
+  int last;               // this workgroup arrived last
+  double sum[kOwnPieces][kPickWaves];
   double border, before;  // random number times the whole mass; mass before the piece
-  int piece, residual, token, tail;
+  int piece, residual;
 };
 
-// A sequence's accepted drafts, and the row its next token comes from: left in
-// sm.choice. Every workgroup of the sequence comes to the same result; `writes`
-// one of them writes it out.
+// A sequence's number of accepted drafts, and the row that its next token comes
+// from, left in sm.choice. Every workgroup of the sequence comes to the same.
 template <typename T, typename Q>
-__device__ __forceinline__ void decide(const VerifyParams& p, VerifySmem& sm, int seq, int begin, int n, bool writes) {
+__device__ __forceinline__ int decide(const VerifyParams& p, VerifySmem& sm, int seq, int begin, int n, float t) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   if (threadIdx.x == 0) sm.first = n;
   __syncthreads();
-  const float t = temperature_of(p, seq);
   float c_hi = 0.f, c_lo = 0.f;
   if (t > 0.f) factor(t, c_hi, c_lo);
   const T* logits = static_cast<const T*>(p.logits);
   const Q* probs = static_cast<const Q*>(p.draft_probs);
-  for (int j = wave; j <= n; j += kWaves) {
+  // a wave's rows, up to its first that is rejected, or row n
+  RowStat r{};
+  int mine = n + 1, x = -1;
+#pragma unroll 1
+  for (int j = wave; j <= n; j += kPickWaves) {
     const int64_t row = static_cast<int64_t>(begin) + seq + j;
     // the draft's own values, on their way beside the statistics
-    int x = -1;
+    x = -1;
     float u = 0.f, l = 0.f, q = 1.f;
     if (j < n) {
       x = p.draft_tokens[begin + j];
@@ -282,59 +351,53 @@ __device__ __forceinline__ void decide(const VerifyParams& p, VerifySmem& sm, in
         if (probs) q = elem<Q>::load1(probs + (static_cast<int64_t>(begin) + j) * p.probs_stride + x);
       }
     }
-    const RowStat r = row_stat(p, row, c_hi, c_lo);
-    if (lane == 0) {
-      if (j < kHeldRows) sm.rows[j] = r;
-      if (j < n) {
-        bool ok = false;
-        if (x >= 0 && x < p.vocab) {
-          double w, s = 1.0;
-          if (t > 0.f && r.m > -INFINITY) {
-            w = weight_f64(l, r.m, t);
-            s = r.s;
-          } else {
-            w = x == (r.m > -INFINITY ? r.arg : 0) ? 1.0 : 0.0;
-          }
-          ok = static_cast<double>(u) * static_cast<double>(q) * s < w;
-        }
-        if (!ok) atomicMin(&sm.first, j);
+    r = row_stat(p, row, c_hi, c_lo);
+    bool ok = false;
+    if (x >= 0 && x < p.vocab) {
+      double w, s = 1.0;
+      if (t > 0.f && r.m > -INFINITY) {
+        w = weight_f64(l, r.m, t);
+        s = r.s;
+      } else {
+        w = x == (r.m > -INFINITY ? r.arg : 0) ? 1.0 : 0.0;
       }
+      ok = static_cast<double>(u) * static_cast<double>(q) * s < w;
+    }
+    if (!ok) {
+      mine = j;
+      break;
     }
   }
+  if (lane == 0) atomicMin(&sm.first, mine);
   __syncthreads();
   const int acc = sm.first;
-  if (wave == 0) {
-    const int64_t row = static_cast<int64_t>(begin) + seq + acc;
-    const RowStat r = acc < kHeldRows ? sm.rows[acc] : row_stat(p, row, c_hi, c_lo);
-    if (lane == 0) {
-      Choice c;
-      c.row = row;
-      c.q_row = acc < n && probs ? static_cast<int64_t>(begin) + acc : -1;
-      c.draft = acc < n && !probs ? p.draft_tokens[begin + acc] : -1;
-      c.column = acc;
-      c.m = r.m;
-      c.c_hi = c_hi;
-      c.c_lo = c_lo;
-      c.only = !(r.m > -INFINITY) ? 0 : (t > 0.f ? -1 : r.arg);
-      c.inv_s = 1.0 / r.s;
-      sm.choice = c;
-    }
-  }
-  if (writes) {
-    int32_t* out = p.out + static_cast<int64_t>(seq) * (p.max_drafts + 1);
-    for (int i = threadIdx.x; i <= p.max_drafts; i += kThreads)
-      if (i != acc) out[i] = i < acc ? p.draft_tokens[begin + i] : -1;
-    if (threadIdx.x == 0) p.n_accepted[seq] = acc;
+  if (mine == acc && lane == 0) {
+    Choice c;
+    c.row = static_cast<int64_t>(begin) + seq + acc;
+    c.q_row = acc < n && probs ? static_cast<int64_t>(begin) + acc : -1;
+    c.draft = acc < n && !probs ? x : -1;
+    c.column = acc;
+    c.m = r.m;
+    c.c_hi = c_hi;
+    c.c_lo = c_lo;
+    c.only = !(r.m > -INFINITY) ? 0 : (t > 0.f ? -1 : r.arg);
+    const double inv = 1.0 / r.s;
+    c.s_hi = static_cast<float>(inv);
+    c.s_lo = static_cast<float>(inv - static_cast<double>(c.s_hi));
+    sm.choice = c;
   }
   __syncthreads();
+  return acc;
 }
 
-// The token: the piece that the border falls into, then the place in it.
-template <typename T, typename Q>
-__device__ __forceinline__ int pick(const VerifyParams& p, VerifySmem& sm, int seq) {
+// The token: the piece that the border falls into, the wave's share of it, the
+// place in that.
+template <typename T, typename Q, bool TINY>
+__device__ __forceinline__ void pick(const VerifyParams& p, VerifySmem& sm, int seq, int32_t* out) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const Choice c = sm.choice;
   if (wave == 0) {
+    const double u = static_cast<double>(p.sample_u[seq]);
     double* mass = p.mass + static_cast<int64_t>(seq) * p.n_pieces;
     const PieceStat* st = static_cast<const PieceStat*>(p.stats) + c.row * p.n_pieces;
     // written by this launch's workgroups where something is subtracted (read past this XCD's L2)
@@ -343,138 +406,139 @@ __device__ __forceinline__ int pick(const VerifyParams& p, VerifySmem& sm, int s
       if (i >= p.n_pieces) return 0.0;
       if (residual) return __hip_atomic_load(mass + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       const PieceStat a = st[i];
-      return a.m > -INFINITY ? a.s * static_cast<double>(weight(a.m, c.m, c.c_hi, c.c_lo)) * c.inv_s : 0.0;
+      return a.m > -INFINITY ? a.s * (static_cast<double>(weight(a.m, c.m, c.c_hi, c.c_lo)) * c.s_hi) : 0.0;
     };
-    auto total_of = [&]() {
-      double s = 0.0;
-      for (int i = lane; i < p.n_pieces; i += kWave) s += piece_mass(i);
-      return wave_sum_f64(s);
-    };
-    double total = total_of();
-    if (residual && !(total > 0.0)) {
-      residual = false;
-      total = total_of();
+    double w0 = 0.0, total = 0.0;  // w0: of this lane's first piece
+#pragma unroll 1
+    for (;;) {
+      w0 = piece_mass(lane);
+      total = w0;
+#pragma unroll 1
+      for (int i = kWave + lane; i < p.n_pieces; i += kWave) total += piece_mass(i);
+      total = wave_sum_f64(total);
+      if (!residual || total > 0.0) break;
+      residual = false;  // nothing is left of p: all of it
     }
-    const double border = static_cast<double>(p.sample_u[seq]) * total;
+    const double border = u * total;
     // the first piece whose running mass exceeds the border; the last one with
     // any mass where none does (u of 1 or more, NaN, or the sums' last bits)
-    int piece = -1, last = -1;
-    double before = 0.0, run = 0.0, last_before = 0.0;
-    for (int i0 = 0; i0 < p.n_pieces && piece < 0; i0 += kWave) {
-      const double w = piece_mass(i0 + lane);
+    int piece = 0;
+    double before = 0.0, run = 0.0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < p.n_pieces; i0 += kWave) {
+      const double w = i0 == 0 ? w0 : piece_mass(i0 + lane);
       const double sum = run + wave_scan_f64(w);
       const uint64_t over = __builtin_amdgcn_ballot_w64(w > 0.0 && sum > border);
       const uint64_t any = __builtin_amdgcn_ballot_w64(w > 0.0);
-      if (over) {
-        const int at = __builtin_ctzll(over);
+      if (any) {
+        const int at = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
         piece = i0 + at;
-        before = __shfl(sum, at, kWave) - __shfl(w, at, kWave);
-      } else if (any) {
-        const int at = 63 - __builtin_clzll(any);
-        last = i0 + at;
-        last_before = __shfl(sum, at, kWave) - __shfl(w, at, kWave);
+        before = lane_f64(sum - w, at);
       }
-      run = __shfl(sum, kWave - 1, kWave);
+      if (over) break;
+      run = lane_f64(sum, kWave - 1);
     }
     if (lane == 0) {
-      sm.piece = piece >= 0 ? piece : max(last, 0);
-      sm.before = piece >= 0 ? before : last_before;
+      sm.piece = piece;
+      sm.before = before;
       sm.border = border;
       sm.residual = residual;
-      sm.token = INT32_MAX;
-      sm.tail = 0;
     }
   }
   __syncthreads();
-  const bool residual = sm.residual != 0;
   const double border = sm.border;
-  const int64_t first = static_cast<int64_t>(sm.piece) * kVerifyPiece + wave * kWavePiece;
-  double w[kSteps][kLaneTokens], own[kSteps], all = 0.0;
+  const Place<TINY> at(sm.piece * kVerifyPiece + wave * kStepTokens + lane * kLaneTokens, p.vocab);
+  float w[kLaneTokens];
+  double own = 0.0;
+  masses<T, Q>(p, c, at, sm.residual != 0, w);
 #pragma unroll
-  for (int k = 0; k < kSteps; k++) {
-    masses<T, Q>(p, c, first + (k * kWave + lane) * kLaneTokens, residual, w[k]);
-    own[k] = 0.0;
-#pragma unroll
-    for (int e = 0; e < kLaneTokens; e++) own[k] += w[k][e];
-    all += own[k];
-  }
-  all = wave_sum_f64(all);
-  if (lane == 0) sm.sum[wave] = all;
+  for (int e = 0; e < kLaneTokens; e++) own += w[e];
+  const double mine = wave_scan_f64(own);
+  if (lane == kWave - 1) sm.sum[0][wave] = mine;
   __syncthreads();
-  double run = sm.before;
-  for (int i = 0; i < wave; i++) run += sm.sum[i];
-  int mine = INT32_MAX, tail = -1;
+  // the first wave whose running mass exceeds the border has the token; the
+  // last one with any mass where none does
+  const double share = lane < kPickWaves ? sm.sum[0][lane] : 0.0;
+  const double upto = sm.before + wave_scan_f64(share);
+  const uint64_t over = __builtin_amdgcn_ballot_w64(share > 0.0 && upto > border);
+  const uint64_t any = __builtin_amdgcn_ballot_w64(share > 0.0);
+  const int who = over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0;
+  if (wave != who) return;
+  double x = lane_f64(upto - share, who) + (mine - own);
+  int first = INT32_MAX, tail = -1;
 #pragma unroll
-  for (int k = 0; k < kSteps; k++) {
-    const double upto = run + wave_scan_f64(own[k]);
-    double at = upto - own[k];
-    const int i = static_cast<int>(first) + (k * kWave + lane) * kLaneTokens;
-#pragma unroll
-    for (int e = 0; e < kLaneTokens; e++) {
-      at += w[k][e];
-      if (w[k][e] > 0.0) {
-        if (at > border) mine = min(mine, i + e);
-        tail = i + e;
-      }
+  for (int e = 0; e < kLaneTokens; e++) {
+    x += w[e];
+    if (w[e] > 0.0) {
+      tail = at.first + e;
+      if (x > border) first = min(first, tail);
     }
-    run = __shfl(upto, kWave - 1, kWave);
   }
-  if (mine != INT32_MAX) atomicMin(&sm.token, mine);
-  if (tail >= 0) atomicMax(&sm.tail, tail);  // the last token of the piece with any mass
-  __syncthreads();
-  return sm.token != INT32_MAX ? sm.token : sm.tail;
+  first = wave_min_i32(first);
+  tail = -wave_min_i32(-tail);  // the last token with any mass
+  if (lane == 0) *out = first != INT32_MAX ? first : max(tail, 0);
 }
 
-template <typename T, typename Q>
-__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyParams p) {
+template <typename T, typename Q, bool TINY>
+__global__ __launch_bounds__(kPickThreads, 8) void verify_kernel(VerifyParams p) {
   __shared__ VerifySmem sm;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  const int piece = blockIdx.x, seq = blockIdx.y;
+  // this workgroup's pieces: first, first + step, ...
+  const int first = blockIdx.x, step = gridDim.x, seq = blockIdx.y;
   int32_t* out = p.out + static_cast<int64_t>(seq) * (p.max_drafts + 1);
+  const float t = temperature_of(p, seq);
   int begin, n;
   if (!span_of(p, seq, begin, n)) {
-    if (piece == 0) {
-      for (int i = threadIdx.x; i <= p.max_drafts; i += kThreads) out[i] = -1;
+    if (first == 0) {
+#pragma unroll 1
+      for (int i = threadIdx.x; i <= p.max_drafts; i += kPickThreads) out[i] = -1;
       if (threadIdx.x == 0) p.n_accepted[seq] = -1;
     }
     return;
   }
-  if (piece > 0 && (n == 0 || !(temperature_of(p, seq) > 0.f))) return;  // nothing to subtract
-  decide<T, Q>(p, sm, seq, begin, n, piece == 0);
+  if (first > 0 && (n == 0 || !(t > 0.f))) return;  // nothing to subtract
+  const int acc = decide<T, Q>(p, sm, seq, begin, n, t);
   const Choice& c = sm.choice;
-  if (c.only >= 0) {
-    if (piece == 0 && threadIdx.x == 0) out[c.column] = c.only;
-    return;
-  }
-  if (c.q_row < 0 && c.draft < 0) {
-    if (piece > 0) return;
-  } else {
-    double s = 0.0;
-#pragma unroll
-    for (int k = 0; k < kSteps; k++) {
-      double w[kLaneTokens];
-      masses<T, Q>(p, c, static_cast<int64_t>(piece) * kVerifyPiece + wave * kWavePiece + (k * kWave + lane) * kLaneTokens,
-                   true, w);
-#pragma unroll
-      for (int e = 0; e < kLaneTokens; e++) s += w[e];
+  const bool subtract = c.only < 0 && (c.q_row >= 0 || c.draft >= 0);
+  if (first > 0 && !subtract) return;
+  if (subtract) {
+    const Choice mine = c;
+    int count = 0;
+#pragma unroll 2
+    for (int piece = first; piece < p.n_pieces; piece += step, count++) {
+      float w[kLaneTokens];
+      masses<T, Q>(p, mine, Place<TINY>(piece * kVerifyPiece + wave * kStepTokens + lane * kLaneTokens, p.vocab), true, w);
+      const double s = wave_sum_f64(sum8(w));
+      if (lane == 0) sm.sum[count][wave] = s;
     }
-    s = wave_sum_f64(s);
-    if (lane == 0) sm.sum[wave] = s;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      double all = 0.0;
-#pragma unroll
-      for (int w = 0; w < kWaves; w++) all += sm.sum[w];
-      __hip_atomic_store(p.mass + static_cast<int64_t>(seq) * p.n_pieces + piece, all, __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
-      __builtin_amdgcn_s_waitcnt(0);  // the mass is where every XCD reads it before the arrival counts
-      sm.last = __hip_atomic_fetch_add(p.arrivals + seq, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == p.n_pieces - 1;
+#pragma unroll 1
+    for (int i = wave; i < count; i += kPickWaves) {
+      const double all = wave_sum_f64(lane < kPickWaves ? sm.sum[i][lane] : 0.0);
+      if (lane == 0)
+        __hip_atomic_store(p.mass + static_cast<int64_t>(seq) * p.n_pieces + first + i * step, all, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
     }
+    __builtin_amdgcn_s_waitcnt(0);  // the masses are where every XCD reads them before the arrival counts
+    __syncthreads();
+    if (threadIdx.x == 0)
+      sm.last = __hip_atomic_fetch_add(p.arrivals + seq, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == step - 1;
+  }
+  if (first == 0) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i <= p.max_drafts; i += kPickThreads)
+      if (i != acc) out[i] = i < acc ? p.draft_tokens[begin + i] : -1;
+    if (threadIdx.x == 0) {
+      p.n_accepted[seq] = acc;
+      if (c.only >= 0) out[acc] = c.only;
+    }
+    if (c.only >= 0) return;
+  }
+  if (subtract) {
     __syncthreads();
     if (!sm.last) return;
   }
-  const int token = pick<T, Q>(p, sm, seq);
-  if (threadIdx.x == 0) out[c.column] = token;
+  pick<T, Q, TINY>(p, sm, seq, out + acc);
 }
 
 }  // namespace
@@ -495,15 +559,21 @@ hipError_t verify_drafts(const VerifyParams& in, int logits_dtype, int probs_dty
   p.mass = reinterpret_cast<double*>(ws);
   p.arrivals = reinterpret_cast<int32_t*>(ws + static_cast<size_t>(p.n_seqs) * p.n_pieces * sizeof(double));
   const unsigned pieces = static_cast<unsigned>(p.n_pieces), seqs = static_cast<unsigned>(p.n_seqs);
+  // two workgroups of the second launch fit on a CU
+  const unsigned share = std::min(pieces, std::max({512u / seqs, (pieces + kOwnPieces - 1) / kOwnPieces, 1u}));
   return with_dtype(logits_dtype, [&](auto a) {
     return with_dtype(probs_dtype, [&](auto b) {
       using T = decltype(a);
       using Q = decltype(b);
-      stats_kernel<T><<<dim3(pieces, static_cast<unsigned>(p.max_drafts + 1), seqs), kThreads, 0, stream>>>(p);
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return e;
-      verify_kernel<T, Q><<<dim3(pieces, seqs), kThreads, 0, stream>>>(p);
-      return hipGetLastError();
+      auto launch = [&](auto tiny) {
+        constexpr bool TINY = decltype(tiny)::value;
+        stats_kernel<T, TINY><<<dim3(pieces, static_cast<unsigned>(p.max_drafts + 1), seqs), kThreads, 0, stream>>>(p);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        verify_kernel<T, Q, TINY><<<dim3(share, seqs), kPickThreads, 0, stream>>>(p);
+        return hipGetLastError();
+      };
+      return p.vocab < kLaneTokens ? launch(std::true_type{}) : launch(std::false_type{});
     });
   });
 }
