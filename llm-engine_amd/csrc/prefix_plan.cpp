@@ -29,6 +29,7 @@ using le::PrefixRow;
 constexpr int kMinSharedKeys = 64;    // a shorter common beginning is not worth a pass of its own
 constexpr int kMaxParts = 128;        // partitions of a tile
 constexpr int kCus = 256;             // MI355X
+constexpr int kWideCost = 2;          // time of a wide tile's keys, in narrow ones
 constexpr int kSmallF32 = 256;        // LDS tiles of wide fp32 items up to which narrow ones take their place
 
 int64_t align256(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
@@ -264,7 +265,7 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   }
   if (n_records > INT32_MAX / 2 || n_items * cfg.kv_heads > INT32_MAX) return LE_EUNSUPPORTED;
 
-  // ---- items, longest first ----
+  // ---- items, the longest to run first ----
   struct Placed {
     PrefixItem item;
     const Tile* tile;
@@ -289,9 +290,8 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
       items.push_back(Placed{it, &t});
     }
   }
-  std::stable_sort(items.begin(), items.end(), [](const Placed& a, const Placed& b) {
-    return a.item.key_end - a.item.key_begin > b.item.key_end - b.item.key_begin;
-  });
+  auto cost = [&](const Placed& a) { return static_cast<int64_t>(a.item.key_end - a.item.key_begin) * (wide(*a.tile) ? kWideCost : 1); };
+  std::stable_sort(items.begin(), items.end(), [&](const Placed& a, const Placed& b) { return cost(a) > cost(b); });
 
   // ---- layout and copy ----
   le_prefix_plan out{};
