@@ -209,6 +209,9 @@ int le_shared_prefix_attention(const void* q, le_dtype act_dtype, const void* k_
   if (cfg.kv_dtype != kv_dtype) return LE_EINVAL;
   if (!plan->dev || !q || !k_cache || !v_cache || !out || !std::isfinite(scale) || num_cache_blocks <= 0)
     return LE_EINVAL;
+  // a kernel's offsets within a block are 32-bit
+  const int64_t row_bytes = static_cast<int64_t>(cfg.kv_heads) * cfg.head_dim * (kv_dtype == LE_F32 ? 4 : 2);
+  if (row_bytes * cfg.block_size > UINT32_MAX) return LE_EUNSUPPORTED;
   if (!aligned16({q, k_cache, v_cache, out})) return LE_EUNSUPPORTED;
   const size_t need = le_shared_prefix_workspace_size(plan);
   if (need > 0 && (!workspace || workspace_bytes < need)) return LE_ENOSPACE;

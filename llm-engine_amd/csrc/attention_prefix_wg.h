@@ -47,6 +47,7 @@ constexpr int kKeys = kPrefixTileKeys;  // keys of an LDS tile
 constexpr int kNarrow = kPrefixNarrow;  // columns up to which the waves share keys
 constexpr float kSlack = 8.f;           // log2 units that scores may pass a column's base by
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short bf16raw4 __attribute__((ext_vector_type(4)));
@@ -231,12 +232,12 @@ template <typename KV, int HD> struct Loader {
   const char* kbase;
   const char* vbase;
   const int32_t* ids;
-  int64_t row_bytes, num_blocks;
+  uint32_t row_bytes, block_bytes, num_blocks;  // a block is less than 4 GiB, the caller checks
   int n_keys, wave, bs_shift, last_blk, window;
   int32_t id_now, id_next;  // lane i: block 64 * window + i's id, and 64 further
   uint32_t off[L::IPW];
   struct Stage {  // a tile in flight
-    uint4 k[L::IPW], v[L::IPW];
+    u32x4 k[L::IPW], v[L::IPW];
     uint32_t gone;  // bits 0 and 1: its rows 0-7 and 8-15 have no block
   };
 
@@ -246,8 +247,9 @@ template <typename KV, int HD> struct Loader {
     kbase = static_cast<const char*>(p.k_cache) + static_cast<int64_t>(kvh) * L::ROW;
     vbase = static_cast<const char*>(p.v_cache) + static_cast<int64_t>(kvh) * L::ROW;
     ids = p.ids + it.ids_off;
-    row_bytes = static_cast<int64_t>(p.kv_heads) * L::ROW;
-    num_blocks = p.num_cache_blocks;
+    row_bytes = static_cast<uint32_t>(p.kv_heads) * L::ROW;
+    block_bytes = row_bytes * p.block_size;
+    num_blocks = static_cast<uint32_t>(min(p.num_cache_blocks, static_cast<int64_t>(INT32_MAX) + 1));
     n_keys = it.key_end - it.key_begin;
     bs_shift = __builtin_ctz(p.block_size);
     last_blk = (n_keys - 1) >> bs_shift;
@@ -259,6 +261,11 @@ template <typename KV, int HD> struct Loader {
       const int row = j * L::RPI + lane / L::CPR;
       off[j] = static_cast<uint32_t>((row & 7) * row_bytes) + (((lane % L::CPR) ^ L::f(row)) << 4);
     }
+  }
+  // eight consecutive rows of a block as a buffer: a scalar descriptor, and a
+  // lane's 32-bit offset is all it adds
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows8(const char* base) const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 8 * row_bytes, 0x00027000);
   }
   // requests the tile whose first key, relative to the item's, is rel
   __device__ __forceinline__ void issue(Stage& st, int rel) {
@@ -274,13 +281,14 @@ template <typename KV, int HD> struct Loader {
       // eight keys (past the range: its last eight again)
       const int key = min(rel + wave * 16 + h * 8, (n_keys - 1) & ~7);
       const int id = __builtin_amdgcn_readlane(id_now, (key >> bs_shift) & (kWave - 1));
-      const bool in = id >= 0 && id < num_blocks;
+      const bool in = static_cast<uint32_t>(id) < num_blocks;
       st.gone |= in ? 0u : 1u << h;
-      const int64_t at = ((static_cast<int64_t>(in ? id : 0) << bs_shift) + (key & ((1 << bs_shift) - 1))) * row_bytes;
+      const uint64_t at = static_cast<uint64_t>(in ? id : 0) * block_bytes + (key & ((1 << bs_shift) - 1)) * row_bytes;
+      const auto kr = rows8(kbase + at), vr = rows8(vbase + at);
 #pragma unroll
       for (int j = h * L::IPW / 2; j < (h + 1) * L::IPW / 2; j++) {
-        st.k[j] = ld16(kbase + at + off[j]);
-        st.v[j] = ld16(vbase + at + off[j]);
+        st.k[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, off[j], 0, 0);
+        st.v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, off[j], 0, 0);
       }
     }
   }
@@ -292,8 +300,8 @@ template <typename KV, int HD> struct Loader {
     char* dst = buf + wave * L::IPW * 1024 + lane * 16;
 #pragma unroll
     for (int j = 0; j < L::IPW; j++) {
-      *reinterpret_cast<uint4*>(dst + j * 1024) = st.k[j];
-      *reinterpret_cast<uint4*>(dst + j * 1024 + L::K_BYTES) = st.v[j];
+      *reinterpret_cast<u32x4*>(dst + j * 1024) = st.k[j];
+      *reinterpret_cast<u32x4*>(dst + j * 1024 + L::K_BYTES) = st.v[j];
     }
     if (live < 16 || st.gone != 0) {
 #pragma unroll
@@ -316,11 +324,10 @@ __device__ __forceinline__ void shared_tiles(Loader<KV, HD>& ld, typename Loader
   const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
   ld.stash(a, sm.lds[0], 0);
   for (int t = 0; t < n_tiles; t++) {
-    const int rel = t * kKeys;
     __syncthreads();  // all rows of tile t are there, and tile t - 1 is no longer read
-    if (t + 1 < n_tiles) ld.issue(a, rel + kKeys);
-    tile(sm.lds[t & 1], rel);
-    if (t + 1 < n_tiles) ld.stash(a, sm.lds[(t + 1) & 1], rel + kKeys);
+    if (t + 1 < n_tiles) ld.issue(a, (t + 1) * kKeys);
+    tile(sm.lds[t & 1], t * kKeys);
+    if (t + 1 < n_tiles) ld.stash(a, sm.lds[(t + 1) & 1], (t + 1) * kKeys);
   }
 }
 // A wave's own rows: two tiles in flight beside the one in use (what bounds
@@ -380,20 +387,36 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
     for (int e = 0; e < 16; e++) acc[d][e] = 0.f;
   float base = 0.f, thr = -FLT_MAX, lsum = 0.f;  // thr -FLT_MAX: no key yet
   const float scale = p.scale_log2;
+  // Where a lane's fragments lie in the tile, piece 0's: a piece further on is
+  // an xor away, and so is the other buffer.
+  const int fk = L::f(col), vrow = 4 * half + (l16 >> 2), vpiece = ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1);
+  int k_at = col * L::ROW + ((half ^ fk) << 4);
+  int v_at = vrow * L::ROW + ((vpiece ^ L::f(vrow)) << 4) + (l16 & 1) * 8;
   shared_tiles(ld, first, sm, [&](const char* b, int rel) {
     if (rel > wave_lim) return;
     f32x16 s[U];
-    const int fk = L::f(col);
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int e = 0; e < 16; e++) s[u][e] = 0.f;
+    // 16-bit products go in the order written: each with the read of the
+    // fragment four products on. (Left to it, the compiler reads two fragments
+    // and waits for them.)
+    constexpr int kAhead = 4, N = U * KS;
+    typename M::frag kf[kAhead];
+    auto k_frag = [&](int i) {
+      if constexpr (sizeof(X) == 2) return M::load(&sm.lds[0][0] + (k_at ^ ((i / U) * 32)) + (i % U) * 32 * L::ROW);
+      else return lds_frag<X, KV, HD>(b + ((i % U) * 32 + col) * L::ROW, fk, ((i / U) * 16 + half * 8) * L::ES / 16);
+    };
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++)
+    for (int i = 0; i < kAhead; i++) kf[i] = k_frag(i);
+    if constexpr (sizeof(X) == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        s[u] = M::wide(lds_frag<X, KV, HD>(b + (u * 32 + col) * L::ROW, fk, (ks * 16 + half * 8) * L::ES / 16), qb[ks],
-                       s[u]);
+    for (int i = 0; i < N; i++) {
+      s[i % U] = M::wide(kf[i % kAhead], qb[i / U], s[i % U]);
+      if (i + kAhead < N) kf[i % kAhead] = k_frag(i + kAhead);
+      if constexpr (sizeof(X) == 2) __builtin_amdgcn_sched_barrier(0);
+    }
     settle<X>();
     // accumulator e of a lane is key 8 (e / 4) + 4 half + e % 4
     if (rel + kKeys - 1 > free_lim) {
@@ -424,9 +447,9 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
 #pragma unroll
       for (int d = 0; d < DT; d++) acc[d] *= alpha;
     }
+    if constexpr (std::is_same_v<X, float>) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if constexpr (std::is_same_v<X, float>) {
+      for (int u = 0; u < U; u++) {
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           s[u][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -base));
@@ -441,33 +464,53 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
             acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[u][e], acc[d], 0, 0, 0);
           }
         }
-      } else {
-        typename M::frag pb[2];
+      }
+    } else {
+      // weights g: those of accumulators 8 (g % 2) .. + 7 of s[g / 2]
+      typename M::frag pb[2 * U];
+      auto weights = [&](int g, int e) {
+        const f32x16& x = s[g / 2];
+        const int at = 8 * (g % 2) + e;
+        typename M::pair w;
+        w[0] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[at], scale, -base)));
+        w[1] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[at + 1], scale, -base)));
+        pb[g][e] = w[0];
+        pb[g][e + 1] = w[1];
+        lsum = M::sum2(w, lsum);
+      };
+      // Beside each product: the read of the fragment two products on, and its
+      // share of the next 16 keys' weights.
+      // V^T operand of 16 keys: lane (dim 16 (lane / 16 % 2) + lane % 16,
+      // half) holds the keys of weights g
+      constexpr int kAheadV = 2, NV = 2 * U * DT;
+      typename M::frag vf[kAheadV];
+      auto v_frag = [&](int i) {
+        const int g = i / DT, d = i % DT;
+        const char* vp = &sm.lds[0][0] + L::K_BYTES + 16 * g * L::ROW;
+        const auto lo = lds_read_tr16<KV>(vp + (v_at ^ (d * 64)));
+        const auto hi = lds_read_tr16<KV>(vp + 8 * L::ROW + (v_at ^ (d * 64 + 32)));  // f(row + 8) = f(row) ^ 2
+        return typename M::frag{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      };
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          typename M::pair w;
-          w[0] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -base)));
-          w[1] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e + 1], scale, -base)));
-          pb[e / 8][e % 8] = w[0];
-          pb[e / 8][e % 8 + 1] = w[1];
-          lsum = M::sum2(w, lsum);
+      for (int i = 0; i < kAheadV; i++) vf[i] = v_frag(i);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) weights(0, e);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int g = i / DT, d = i % DT;
+        acc[d] = M::wide(vf[i % kAheadV], pb[g], acc[d]);
+        if (i + kAheadV < NV) vf[i % kAheadV] = v_frag(i + kAheadV);
+        if (g + 1 < 2 * U) {
+#pragma unroll
+          for (int e = d * 8 / DT; e < (d + 1) * 8 / DT; e += 2) weights(g + 1, e);
         }
-        // V^T operand of 16 keys: lane (dim 16 (lane / 16 % 2) + lane % 16,
-        // half) holds the keys of accumulators 8 h .. 8 h + 7
-        const int row = 4 * half + (l16 >> 2), piece = ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1);
-        const int f_lo = L::f(row), f_hi = L::f(row + 8);
-        const char* vp = b + L::K_BYTES + (u * 32 + row) * L::ROW + (l16 & 1) * 8;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-          for (int d = 0; d < DT; d++) {
-            const auto lo = lds_read_tr16<KV>(vp + 16 * h * L::ROW + (((d * 4 + piece) ^ f_lo) << 4));
-            const auto hi = lds_read_tr16<KV>(vp + (16 * h + 8) * L::ROW + (((d * 4 + piece) ^ f_hi) << 4));
-            const typename M::frag va = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            acc[d] = M::wide(va, pb[h], acc[d]);
-          }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
+    k_at ^= L::BYTES;
+    v_at ^= L::BYTES;
   });
 
   // acc[d][e] = O[column][dim 32 d + 8 (e / 4) + 4 half + e % 4]

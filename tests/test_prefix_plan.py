@@ -181,6 +181,16 @@ def test_attention_refusals_without_launch():
     assert L.le_shared_prefix_attention(fake, 1, fake, fake, 1, 1, None, 1.0, fake, fake, 0, nul) == _lib.LE_EINVAL
 
 
+def test_blocks_past_32_bit_offsets_are_refused():
+    plan = pack([(np.arange(30), 400, 1), (np.arange(30), 410, 1)])
+    P, L, fake = plan.plan, _lib.load(), ctypes.c_void_p(4096)
+    P.dev = 4096
+    P.cfg.q_heads = P.cfg.kv_heads = 1 << 15
+    P.cfg.head_dim, P.cfg.block_size = 128, 512  # 2^15 * 128 * 2 bytes * 512 = 4 GiB
+    st = L.le_shared_prefix_attention(fake, 1, fake, fake, 1, 64, ctypes.byref(P), 1.0, fake, fake, 0, None)
+    assert st == _lib.LE_EUNSUPPORTED
+
+
 def test_verify_refusals_without_launch():
     L = _lib.load()
     fake, odd, nul = ctypes.c_void_p(4096), ctypes.c_void_p(4104), ctypes.c_void_p(0)
