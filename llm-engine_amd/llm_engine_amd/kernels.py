@@ -73,6 +73,15 @@ def _bytes(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.numel() * t.element_size()
 
 
+def _empty(stream, size, dtype: torch.dtype, device) -> torch.Tensor:
+    """A tensor from the pool of the stream that the launch goes to: memory that
+    work queued on another one still uses is never handed out."""
+    if stream is None:
+        return torch.empty(size, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(size, dtype=dtype, device=device)
+
+
 def _launch(name: str, device: int, stream, *args) -> None:
     """Calls an entry point whose last argument is the stream, with the tensors'
     device as the current one (their stream: that device's current one)."""
@@ -170,7 +179,7 @@ def qk_norm_rope_store_kv(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
     if bias is not None and not _f32(bias, row, dev):
         raise ValueError("bias: contiguous fp32 cuda [q_dim + 2*kv_dim]")
     if q_out is None:
-        q_out = torch.empty(n, q_heads * head_dim, dtype=qkv.dtype, device=qkv.device)
+        q_out = _empty(stream, (n, q_heads * head_dim), qkv.dtype, qkv.device)
     elif not (q_out.is_contiguous() and q_out.dtype == qkv.dtype and q_out.numel() == n * q_heads * head_dim
               and q_out.get_device() == dev):
         raise ValueError("q_out: contiguous cuda [N, q_heads*head_dim] in qkv's dtype")
@@ -225,16 +234,16 @@ def verify_drafts(logits: torch.Tensor, cu_drafts: torch.Tensor, draft_tokens: t
                                         and draft_probs.get_device() == dev):
         raise ValueError("draft_probs: cuda [drafts, vocab] with unit column stride")
     if out is None:
-        out = torch.empty(n_seqs, max_drafts + 1, dtype=torch.int32, device=logits.device)
+        out = _empty(stream, (n_seqs, max_drafts + 1), torch.int32, logits.device)
     elif not (_i32(out, 0, dev) and out.dim() == 2 and out.size(0) == n_seqs and out.size(1) == max_drafts + 1):
         raise ValueError("out: contiguous int32 cuda [sequences, max_drafts + 1]")
     if n_accepted is None:
-        n_accepted = torch.empty(n_seqs, dtype=torch.int32, device=logits.device)
+        n_accepted = _empty(stream, (n_seqs,), torch.int32, logits.device)
     elif not _i32(n_accepted, n_seqs, dev):
         raise ValueError("n_accepted: contiguous int32 cuda [sequences]")
     need = _lib.load().le_verify_drafts_workspace_size(n_seqs, n_drafts, vocab)
     if _bytes(workspace) < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        workspace = _empty(stream, (need,), torch.uint8, logits.device)
     elif workspace is not None and workspace.get_device() != dev:
         raise ValueError("workspace: on the tensors' device")
     _launch("le_verify_drafts", dev, stream, logits.data_ptr(), _dt(logits), _row_stride(logits), vocab,
@@ -484,10 +493,13 @@ class PrefixPlan:
 
     def upload(self, stream=None) -> "PrefixPlan":
         nbytes = int(self.plan.bytes)
-        if self.device_buf is None or self.device_buf.numel() < nbytes:
-            self.device_buf = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        _launch("le_prefix_plan_upload", self.device_buf.get_device(), stream, ctypes.byref(self.plan),
-                self.host.data_ptr(), self.device_buf.data_ptr())
+        if self.device_buf is None:
+            self.device_buf = _empty(stream, (nbytes,), torch.uint8, self.device)
+        # torch's own copy (le_prefix_plan_upload's, but torch knows of it): the
+        # pinned buffer of a plan that is dropped is not reused before it ends
+        with torch.cuda.stream(stream):
+            self.device_buf.copy_(self.host, non_blocking=True)
+        self.plan.dev = self.device_buf.data_ptr()
         return self
 
     @property
@@ -522,11 +534,11 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
             and k_cache.get_device() == v_cache.get_device() == dev):
         raise ValueError("k_cache, v_cache: contiguous cuda, alike, whole blocks")
     if out is None:
-        out = torch.empty_like(q)
+        out = _empty(stream, q.shape, q.dtype, q.device)
     elif not (out.dtype == q.dtype and out.numel() == q.numel() and out.is_contiguous() and out.get_device() == dev):
         raise ValueError("out: like q")
     if _bytes(workspace) < plan._need:
-        workspace = torch.empty(plan._need, dtype=torch.uint8, device=q.device)
+        workspace = _empty(stream, (plan._need,), torch.uint8, q.device)
     elif workspace is not None and workspace.get_device() != dev:
         raise ValueError("workspace: on the tensors' device")
     _launch("le_shared_prefix_attention", dev, stream, q.data_ptr(), _dt(q), k_cache.data_ptr(), v_cache.data_ptr(),
