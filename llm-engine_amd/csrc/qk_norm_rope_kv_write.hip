@@ -8,9 +8,16 @@
 // A head is held by head_dim / (2 W) adjacent lanes: a lane has W elements of
 // its lower half and the W that they rotate with (W = 8: two 16-byte pieces
 // of a 16-bit row), so the mean is one reduction inside the wave, and neither
-// the norm nor the rotation goes through memory. One workgroup takes a token;
-// a lane's dims are the same for all its heads, so its cos, sin and norm
-// weights stay in registers.
+// the norm nor the rotation goes through memory. A lane's dims are the same for
+// all its heads, so its cos and sin stay in registers.
+//
+// Bound by the bytes of the rows. A workgroup takes a token, all heads; while
+// all workgroups run at once anyway, several share a token, a head per lane
+// group, so that no second head waits for the first one's trip to memory (32 +
+// 2 x 8 heads of 128, 15 fp32 rows: 3.2 us, unshared 4.1; 905 fp16 rows 8.1,
+// 8.6). Past that the copies of cos and sin cost more (1371 fp32 rows: 14.3 us,
+// 15.1 shared). 4096 bf16 rows of that shape take 24.5 us, 4.2 TB/s, where a
+// copy of 1 GiB reaches 5.0; 3898 rows of 10 + 2 x 10 heads 4.99 TB/s.
 #include "le_common.h"
 #include "le_internal.h"
 
@@ -18,6 +25,7 @@ namespace le {
 namespace {
 
 constexpr int kNormThreads = 256;
+constexpr int kResident = 2048;  // workgroups that run at once: 256 CUs of 32 waves
 
 template <typename T, int W> __device__ __forceinline__ void load_w(const T* p, float* o) {
   if constexpr (W == 8) elem<T>::load8(p, o);
@@ -35,7 +43,7 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_kernel(QkNormParams
   const int lanes = LANES > 0 ? LANES : p.lanes;
   const int t = blockIdx.x;
   const int hd = LANES > 0 ? 2 * W * LANES : p.head_dim, half = hd >> 1;
-  const int unit0 = threadIdx.x / lanes, per_step = kNormThreads / lanes;
+  const int unit0 = (blockIdx.y * kNormThreads + threadIdx.x) / lanes, per_step = gridDim.y * kNormThreads / lanes;
   const int i = (threadIdx.x & (lanes - 1)) * W;  // this lane's dims: [i, i + W) and the same past half
   const bool live = LANES > 0 || i < half;
   const int at = live ? i : 0;
@@ -104,19 +112,22 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_kernel(QkNormParams
 
 hipError_t qk_norm_rope_kv_write(const QkNormParams& in, int act_dtype, int cache_dtype, hipStream_t stream) {
   QkNormParams p = in;
-  const dim3 grid(static_cast<unsigned>(p.n_tokens));
+  const auto grid = [&](int lanes) {
+    const int64_t split = (static_cast<int64_t>(p.q_heads + 2 * p.kv_heads) * lanes + kNormThreads - 1) / kNormThreads;
+    return dim3(static_cast<unsigned>(p.n_tokens), p.n_tokens * split <= kResident ? static_cast<unsigned>(split) : 1u);
+  };
   return with_dtype(act_dtype, [&](auto a) {
     return with_dtype(cache_dtype, [&](auto c) {
       using T = decltype(a);
       using C = decltype(c);
       if (p.head_dim == 64) {
-        qk_norm_rope_kernel<T, C, 8, 4><<<grid, kNormThreads, 0, stream>>>(p);
+        qk_norm_rope_kernel<T, C, 8, 4><<<grid(4), kNormThreads, 0, stream>>>(p);
       } else if (p.head_dim == 128) {
-        qk_norm_rope_kernel<T, C, 8, 8><<<grid, kNormThreads, 0, stream>>>(p);
+        qk_norm_rope_kernel<T, C, 8, 8><<<grid(8), kNormThreads, 0, stream>>>(p);
       } else {
         p.lanes = 1;
         while (p.lanes * 8 < p.head_dim) p.lanes *= 2;
-        qk_norm_rope_kernel<T, C, 4, 0><<<grid, kNormThreads, 0, stream>>>(p);
+        qk_norm_rope_kernel<T, C, 4, 0><<<grid(p.lanes), kNormThreads, 0, stream>>>(p);
       }
       return hipGetLastError();
     });
