@@ -462,13 +462,14 @@ int le_add_bias(void* x, le_dtype dtype, const float* bias, int rows, int cols, 
  * A temperature of 0 or less (or NaN) is greedy: p is 1 at the row's first
  * maximum. A logit that is NaN or -inf has probability 0, several of +inf share
  * it; a row with nothing above -inf has p 1 at token 0. A draft outside
- * [0, vocab) is rejected. Random numbers are in [0, 1); 1 or more, or NaN, never
- * accepts, and samples the last token with any mass. Sums and comparisons are
- * fp64 over fp32 weights.
+ * [0, vocab) is rejected. Random numbers are in [0, 1); a NaN never accepts, and
+ * a sample_u of 1 or more, or NaN, gives the last token with any mass. Sums and
+ * comparisons are fp64 over fp32 weights.
  * out[s] = [accepted drafts..., the sampled token, -1...], max_drafts + 1
  * entries; n_accepted[s] the number of accepted drafts. Offsets that decrease,
  * leave [0, n_drafts] or hold more than max_drafts give out[s] = -1... and
- * n_accepted[s] = -1. Rows may start at any element; the workspace is 16-byte
+ * n_accepted[s] = -1 (other sequences are right as long as their drafts do not
+ * overlap). Rows may start at any element; the workspace is 16-byte
  * aligned, needs no clearing, and is used by one call at a time.
  * ------------------------------------------------------------------------ */
 size_t le_verify_drafts_workspace_size(int n_seqs, int n_drafts, int vocab);

@@ -20,8 +20,9 @@
 // second has several workgroups for a sequence, about two a CU in all: each
 // forms the decision from the rows' piece statistics (some KB; a launch of its
 // own for it costs more), then the masses of its pieces of max(p - q, 0); the
-// last one to arrive picks the token. A row without drafts' probabilities to subtract has its
-// pieces' masses in the statistics already: its first workgroup picks alone.
+// last one to arrive picks the token. A row without a draft's probabilities to
+// subtract has its pieces' masses in the statistics already: its first workgroup
+// picks alone, after it has summed the piece of a rejected token without it.
 //
 // The second launch is a chain of short steps, each run once: what bounds it is
 // how many memory round trips and cross-lane reductions follow each other, and
@@ -375,7 +376,7 @@ __device__ __forceinline__ int decide(const VerifyParams& p, VerifySmem& sm, int
     Choice c;
     c.row = static_cast<int64_t>(begin) + seq + acc;
     c.q_row = acc < n && probs ? static_cast<int64_t>(begin) + acc : -1;
-    c.draft = acc < n && !probs ? x : -1;
+    c.draft = acc < n && !probs && x < p.vocab ? x : -1;
     c.column = acc;
     c.m = r.m;
     c.c_hi = c_hi;
@@ -400,13 +401,17 @@ __device__ __forceinline__ void pick(const VerifyParams& p, VerifySmem& sm, int 
     const double u = static_cast<double>(p.sample_u[seq]);
     double* mass = p.mass + static_cast<int64_t>(seq) * p.n_pieces;
     const PieceStat* st = static_cast<const PieceStat*>(p.stats) + c.row * p.n_pieces;
-    // written by this launch's workgroups where something is subtracted (read past this XCD's L2)
     bool residual = c.q_row >= 0 || c.draft >= 0;
+    const int less = c.draft >= 0 ? c.draft / kVerifyPiece : -1;  // the rejected token's piece, summed without it
+    const double rest = less >= 0 ? wave_sum_f64(lane < kPickWaves ? sm.sum[0][lane] : 0.0) : 0.0;
+    const double inv = static_cast<double>(c.s_hi) + static_cast<double>(c.s_lo);
     auto piece_mass = [&](int i) {
       if (i >= p.n_pieces) return 0.0;
-      if (residual) return __hip_atomic_load(mass + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      // written by this launch's workgroups (read past this XCD's L2)
+      if (residual && c.q_row >= 0) return __hip_atomic_load(mass + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (residual && i == less) return rest;
       const PieceStat a = st[i];
-      return a.m > -INFINITY ? a.s * (static_cast<double>(weight(a.m, c.m, c.c_hi, c.c_lo)) * c.s_hi) : 0.0;
+      return a.m > -INFINITY ? a.s * (static_cast<double>(weight(a.m, c.m, c.c_hi, c.c_lo)) * inv) : 0.0;
     };
     double w0 = 0.0, total = 0.0;  // w0: of this lane's first piece
 #pragma unroll 1
@@ -499,7 +504,7 @@ __global__ __launch_bounds__(kPickThreads, 8) void verify_kernel(VerifyParams p)
   if (first > 0 && (n == 0 || !(t > 0.f))) return;  // nothing to subtract
   const int acc = decide<T, Q>(p, sm, seq, begin, n, t);
   const Choice& c = sm.choice;
-  const bool subtract = c.only < 0 && (c.q_row >= 0 || c.draft >= 0);
+  const bool subtract = c.only < 0 && c.q_row >= 0;
   if (first > 0 && !subtract) return;
   if (subtract) {
     const Choice mine = c;
@@ -523,6 +528,15 @@ __global__ __launch_bounds__(kPickThreads, 8) void verify_kernel(VerifyParams p)
     __syncthreads();
     if (threadIdx.x == 0)
       sm.last = __hip_atomic_fetch_add(p.arrivals + seq, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == step - 1;
+  }
+  if (c.only < 0 && c.draft >= 0) {
+    const Choice mine = c;
+    float w[kLaneTokens];
+    const int piece = mine.draft / kVerifyPiece;
+    masses<T, Q>(p, mine, Place<TINY>(piece * kVerifyPiece + wave * kStepTokens + lane * kLaneTokens, p.vocab), true, w);
+    const double s = wave_sum_f64(sum8(w));
+    if (lane == 0) sm.sum[0][wave] = s;
+    __syncthreads();
   }
   if (first == 0) {
 #pragma unroll 1
@@ -560,7 +574,7 @@ hipError_t verify_drafts(const VerifyParams& in, int logits_dtype, int probs_dty
   p.arrivals = reinterpret_cast<int32_t*>(ws + static_cast<size_t>(p.n_seqs) * p.n_pieces * sizeof(double));
   const unsigned pieces = static_cast<unsigned>(p.n_pieces), seqs = static_cast<unsigned>(p.n_seqs);
   // two workgroups of the second launch fit on a CU
-  const unsigned share = std::min(pieces, std::max({512u / seqs, (pieces + kOwnPieces - 1) / kOwnPieces, 1u}));
+  const unsigned share = p.draft_probs ? std::min(pieces, std::max({512u / seqs, (pieces + kOwnPieces - 1) / kOwnPieces, 1u})) : 1u;
   return with_dtype(logits_dtype, [&](auto a) {
     return with_dtype(probs_dtype, [&](auto b) {
       using T = decltype(a);

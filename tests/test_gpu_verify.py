@@ -174,6 +174,31 @@ def test_residual_without_mass_falls_back(gpu):
     c.check()
 
 
+@pytest.mark.parametrize("vocab", [5, 8192, 8193, 30011])
+def test_rejected_lookup_drafts(gpu, vocab):
+    """Drafts without probabilities that are rejected: at a piece's ends, with
+    nearly all of the row's mass, alone in their piece, alone in the row (sampled
+    after all), and with nothing of their own."""
+    at = [0, vocab // 2, vocab - 1, min(8191, vocab - 1), min(8192, vocab - 1), vocab - 2, 3, 1]
+    c = Case([1] * 8, vocab, "f32", None, seed=40 + vocab)
+    c.tokens[:] = torch.tensor(at, dtype=torch.int32)
+    c.au.fill_(1.0 - 2.0 ** -24)
+    x = c.logits
+    for i in range(3):
+        x[2 * i, at[i]] = 30.0                     # e^30 against about vocab e^8 at most
+    for i in (3, 4):                               # the piece's only token
+        lo = at[i] // 8192 * 8192
+        keep = x[2 * i, at[i]].clone()
+        x[2 * i, lo:lo + 8192] = -math.inf
+        x[2 * i, at[i]] = keep
+    x[10] = -math.inf
+    x[10, at[5]] = 1.0
+    x[12, at[6]] = -math.inf
+    x[14, at[7]] = math.nan
+    acc = c.check().tolist()
+    assert acc[6] == acc[7] == 0
+
+
 def test_bad_tokens_offsets_and_random_numbers(gpu):
     c = Case([2, 3, 1, 2], 2500, seed=11)
     c.tokens[0], c.tokens[3] = -1, 2500            # no such tokens: rejected
