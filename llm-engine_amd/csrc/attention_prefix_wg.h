@@ -720,7 +720,7 @@ __global__ __launch_bounds__(kThreads, (std::is_same_v<operand<ACT, KV>, float> 
 // ---- rows of several parts: a wave for each (row, head) ----
 // The parts' factors are formed by the lanes together (a part each, 64 at a
 // time); then a lane has four dims of every 64 / (HD / 4)-th part, four loads in
-// flight. (One thread per four dims that went through all parts by itself took
+// flight beside the four in use. (One thread per four dims that went through all parts by itself took
 // 21.7 us for 64 rows x 14 heads x 64 of 34 parts.)
 template <typename ACT, int HD>
 __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(PrefixParams p) {
@@ -736,29 +736,34 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(PrefixParams p) 
   const float* acc = p.acc + rec0 * HD + (lane & (DL - 1)) * 4;
   const int64_t step = static_cast<int64_t>(p.q_heads) * HD;
   const int group = lane / DL;
-  float M = -FLT_MAX;
-  for (int k = lane; k < n; k += kWave) M = fmaxf(M, ml[static_cast<int64_t>(k) * p.q_heads].x);
+  // the parts' factors, 64 at a time, and beside them the first parts' loads
+  float2 x = ml[static_cast<int64_t>(min(lane, n - 1)) * p.q_heads];
+  f32x4 v[4];
+  auto load = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const f32x4*>(acc + min(k + j * GROUPS + group, n - 1) * step);
+  };
+  load(0);
+  float M = x.x;
+  for (int k = lane + kWave; k < n; k += kWave) M = fmaxf(M, ml[static_cast<int64_t>(k) * p.q_heads].x);
   M = wave_max(M);
   float l = 0.f;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
   for (int k0 = 0; k0 < n; k0 += kWave) {
-    const int last = min(n - k0, kWave) - 1;  // of these parts
-    const float2 x = ml[static_cast<int64_t>(k0 + min(lane, last)) * p.q_heads];
-    const float f = lane <= last ? __builtin_amdgcn_exp2f(x.x - M) : 0.f;
+    if (k0 > 0) x = ml[static_cast<int64_t>(min(k0 + lane, n - 1)) * p.q_heads];
+    const float f = k0 + lane < n ? __builtin_amdgcn_exp2f(x.x - M) : 0.f;
     l += x.y * f;
-    for (int i = 0; i <= last; i += 4 * GROUPS) {  // (all lanes: a part's factor may be any lane's)
-      const int k = i + group;
-      f32x4 v[4];
-      float w[4];
+    const int end = min(n - k0, kWave);
+    for (int i = 0; i < end; i += 4 * GROUPS) {  // (all lanes: a part's factor may be any lane's)
+      f32x4 now[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) now[j] = v[j];
+      if (k0 + i + 4 * GROUPS < n) load(k0 + i + 4 * GROUPS);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int at = min(k + j * GROUPS, last);
-        v[j] = *reinterpret_cast<const f32x4*>(acc + (k0 + at) * step);
-        w[j] = __shfl(f, at, kWave);
-        if (k + j * GROUPS > last) w[j] = 0.f;
+        const float w = __shfl(f, i + j * GROUPS + group, kWave);
+        a += w > 0.f ? now[j] * w : f32x4{0.f, 0.f, 0.f, 0.f};
       }
-#pragma unroll
-      for (int j = 0; j < 4; j++) a += w[j] > 0.f ? v[j] * w[j] : f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
   l = wave_sum(l);
