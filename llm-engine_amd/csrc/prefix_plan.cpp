@@ -34,6 +34,15 @@ constexpr int kSmallF32 = 256;        // LDS tiles of wide fp32 items up to whic
 
 int64_t align256(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
 
+// the number of ids, up to n, that two tables begin with alike
+int common(const int32_t* a, const int32_t* b, int n) {
+  constexpr int kRun = 64;
+  int i = 0;
+  while (i + kRun <= n && std::memcmp(a + i, b + i, kRun * sizeof(int32_t)) == 0) i += kRun;
+  while (i < n && a[i] == b[i]) i++;
+  return i;
+}
+
 struct Group {
   int first, count;  // among the sorted slices
   int blocks;        // shared blocks
@@ -158,14 +167,13 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
     order[i] = i;
   }
   std::stable_sort(order.begin(), order.end(), [&](int a, int b) {
-    return std::lexicographical_compare(table[a]->blocks, table[a]->blocks + cap[a], table[b]->blocks,
-                                        table[b]->blocks + cap[b]);
+    const int m = std::min(cap[a], cap[b]), at = common(table[a]->blocks, table[b]->blocks, m);
+    return at < m ? table[a]->blocks[at] < table[b]->blocks[at] : cap[a] < cap[b];
   });
   std::vector<int> lcp(n_slices, 0);
   for (int i = 1; i < n_slices; i++) {
-    const int a = order[i - 1], b = order[i], m = std::min(cap[a], cap[b]);
-    lcp[i] = static_cast<int>(
-        std::mismatch(table[a]->blocks, table[a]->blocks + m, table[b]->blocks).first - table[a]->blocks);
+    const int a = order[i - 1], b = order[i];
+    lcp[i] = common(table[a]->blocks, table[b]->blocks, std::min(cap[a], cap[b]));
   }
   const std::vector<Group> groups = best_groups(lcp, std::max(1, (kMinSharedKeys + bs - 1) / bs));
 

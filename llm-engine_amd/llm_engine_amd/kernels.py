@@ -477,14 +477,15 @@ class PrefixPlan:
             arr[i] = StepSlice(s.seq_key, s.start, s.len, int(s.needs_logits), b.size, b.ctypes.data, None)
         self.plan = PrefixStepPlan()
         L = _lib.load()
-        st = L.le_prefix_plan_step(arr, len(slices), ctypes.byref(self.cfg), None, 0, ctypes.byref(self.plan))
-        if st != _lib.LE_ENOSPACE:  # (an empty step needs no buffer)
-            check("le_prefix_plan_step", st)
-        nbytes = int(self.plan.bytes)
-        self.host = torch.empty(nbytes, dtype=torch.uint8, pin_memory=pin and torch.cuda.is_available())
-        check("le_prefix_plan_step", L.le_prefix_plan_step(arr, len(slices), ctypes.byref(self.cfg),
-                                                           ctypes.c_void_p(self.host.data_ptr()), nbytes,
-                                                           ctypes.byref(self.plan)))
+        nbytes = (256 << 10) + (len(slices) << 10)  # room for most steps: packed at once, not sized first
+        while True:
+            self.host = torch.empty(nbytes, dtype=torch.uint8, pin_memory=pin and torch.cuda.is_available())
+            st = L.le_prefix_plan_step(arr, len(slices), ctypes.byref(self.cfg),
+                                       ctypes.c_void_p(self.host.data_ptr()), nbytes, ctypes.byref(self.plan))
+            if st != _lib.LE_ENOSPACE or self.plan.bytes <= nbytes:
+                break
+            nbytes = int(self.plan.bytes)
+        check("le_prefix_plan_step", st)
         self._need = int(L.le_shared_prefix_workspace_size(ctypes.byref(self.plan)))
         self._block = block_size * kv_heads * head_dim
         self._q_numel = int(self.plan.n_tokens) * q_heads * head_dim
@@ -498,7 +499,7 @@ class PrefixPlan:
         # torch's own copy (le_prefix_plan_upload's, but torch knows of it): the
         # pinned buffer of a plan that is dropped is not reused before it ends
         with torch.cuda.stream(stream):
-            self.device_buf.copy_(self.host, non_blocking=True)
+            self.device_buf.copy_(self.host[:nbytes], non_blocking=True)
         self.plan.dev = self.device_buf.data_ptr()
         return self
 

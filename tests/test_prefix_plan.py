@@ -162,6 +162,21 @@ def test_packer_refusals():
         pack([(t, 64, 1)])
 
 
+def test_plans_larger_than_the_first_buffer():
+    plan = pack([(np.arange(100_000), 800_000 - 1, 1)], block=8)  # 400 KB of ids
+    assert plan.plan.bytes > 400_000 and plan.host.numel() >= plan.plan.bytes
+    assert (arrays(plan)[3][:100_000] == np.arange(100_000)).all()
+
+
+@pytest.mark.parametrize("differ", [0, 63, 64, 65, 127, 128, 190])
+def test_common_beginnings_of_any_length(differ):
+    """Two tables of 200 ids that differ at one place share what is before it."""
+    a, b = np.arange(200), np.arange(200)
+    b[differ] = 1000
+    plan = check([(a, 1600 - 1, 1), (b, 1600 - 1, 1)], block=8)
+    assert plan.saved_keys == (8 * differ if 8 * differ >= 64 else 0)
+
+
 def test_attention_refusals_without_launch():
     plan = pack([(np.arange(30), 400, 1), (np.arange(30), 410, 1)])
     P, L = plan.plan, _lib.load()
