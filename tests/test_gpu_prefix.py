@@ -186,6 +186,48 @@ def test_numbers_of_parts(gpu, heads):
     Step([(0, 8, k, 1) for k in own], heads, seed=20, partition_tokens=64, chunk_partition_tokens=128).check()
 
 
+@pytest.mark.parametrize("tile", [32, 128])
+@pytest.mark.parametrize("heads,kv", [(QWEN, "bf16"), (QWEN, "f32"), (WIDE, "f16"), (WIDE, "f32"), ((3, 3, 128), "bf16")])
+def test_tile_widths(gpu, heads, kv, tile):
+    """Tiles of at most 32 columns, or up to 128, asked for."""
+    seqs = BATCH + [(0, 20, 90, 50), (1, 5, 64, 8), (1, 5, 3, 2), (2, 0, 140, 140)]
+    Step(seqs, heads, act=kv, kv=kv, seed=21, chunk_q_tile=tile).check()
+
+
+@pytest.mark.parametrize("heads,kv", [(QWEN, "bf16"), (WIDE, "f16"), (QWEN, "f32")])
+def test_more_block_ids_than_lanes(gpu, heads, kv):
+    """Items of several times 64 blocks, in wide tiles and in narrow ones."""
+    seqs = [(0, 333, 5, 1)] * 9 + [(1, 0, 8 * 197 + 3, 1), (2, 0, 8 * 130, 40), (3, 64, 8, 8), (3, 64, 9, 9)]
+    Step(seqs, heads, act=kv, kv=kv, block=8, seed=22, partition_tokens=100000, chunk_partition_tokens=100000,
+         chunk_q_tile=128).check()
+
+
+@pytest.mark.parametrize("kv", ["bf16", "f32"])
+def test_nan_and_infinities_stay_with_their_rows(gpu, kv):
+    """A q row, a key and a value of one sequence: the rows and heads that the
+    formula makes NaN are, and no other output changes a bit."""
+    s = Step(BATCH + [(0, 20, 60, 30)], QWEN, act=kv, kv=kv, seed=23)
+    clean, G, d = s.run(), s.H // s.KH, s.d
+    s.q[3, 2 * d + 1] = math.nan                                    # row 3, head 2
+    s.k[s.slots(5)[s.keys[5] - 2], d + 4] = math.inf                # sequence 5, kv head 1
+    s.v[s.slots(6)[s.keys[6] - 30], 9] = math.nan                   # sequence 6, kv head 0, dim 9
+    s.q[8, 13 * d:] = -math.inf                                     # row 8, the last head
+    got = s.run()
+    want, _ = s.want()
+    bad = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), bad)
+    # where q's sign makes the infinite key score -inf, it drops out: no NaN,
+    # and off by at most 2 w max|v| and one rounding (w as above, 1e-3 for the scores)
+    drop = torch.zeros_like(bad)
+    drop[5, G * d:] = ~bad[5, G * d:]
+    assert bool(bad[5, G * d:].any()) and bool(drop.any())
+    tol = (3 * HALF_STEP[s.q.dtype] + 1e-3) * float(s.v.float().nan_to_num().abs().max())
+    assert float((got.double() - want)[drop].abs().max()) <= tol
+    heads = (bad | drop).reshape(-1, s.H, d).any(-1).nonzero().tolist()
+    assert heads == [[3, 2]] + [[5, h] for h in range(G, s.H)] + [[6, h] for h in range(G)] + [[8, 13]]
+    assert torch.equal(got[~(bad | drop)], clean[~(bad | drop)])
+
+
 @pytest.mark.parametrize("kv", ["bf16", "f16", "f32"])
 def test_dead_cache_rows_are_not_read(gpu, kv):
     """NaN in every cache row that no sequence has computed (the rest of the last

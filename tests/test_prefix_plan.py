@@ -177,6 +177,23 @@ def test_common_beginnings_of_any_length(differ):
     assert plan.saved_keys == (8 * differ if 8 * differ >= 64 else 0)
 
 
+@pytest.mark.parametrize("seed", range(12))
+def test_random_steps_in_asked_tiles(seed):
+    rng = np.random.default_rng(100 + seed)
+    tables = [rng.integers(0, 500, 60) for _ in range(3)]
+    seqs = []
+    for _ in range(int(rng.integers(1, 30))):
+        depth, own = int(rng.integers(0, 50)), int(rng.integers(1, 40))
+        table = np.concatenate([tables[rng.integers(0, 3)][:depth], rng.integers(500, 900, own)])
+        rows = int(rng.integers(1, 1 + min(60, 16 * len(table))))
+        seqs.append((table, 16 * len(table) - rows - int(rng.integers(0, min(15, 16 * len(table) - rows) + 1)), rows))
+    heads = [(14, 2, 64), (32, 8, 128), (8, 1, 64), (5, 5, 64)][seed % 4]
+    tile = 32 if seed % 2 else 128
+    plan = check(seqs, heads, chunk_q_tile=tile, partition_tokens=int(rng.integers(0, 300)),
+                 chunk_partition_tokens=int(rng.integers(0, 900)))
+    assert (arrays(plan)[0][:, 0] * (heads[0] // heads[1]) <= tile).all()
+
+
 def test_attention_refusals_without_launch():
     plan = pack([(np.arange(30), 400, 1), (np.arange(30), 410, 1)])
     P, L = plan.plan, _lib.load()
