@@ -185,8 +185,8 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
     const int n = static_cast<int>(rows.size());
     // fp32 products take 3.6 us per 64 keys (head_dim 64) in a wide tile and
     // 0.9 in a narrow one: a step too small to fill the chip with wide ones is
-    // cut into narrow ones (24 rows behind 1500 keys, 14/2 heads x 64: 12.3 us
-    // against 14.1; 128 rows behind 4096: 42.6 against 34.7).
+    // cut into narrow ones (24 rows behind 1500 keys, 14/2 heads x 64: 12.0 us
+    // against 13.4; 128 rows behind 4096: 116 against 36).
     const int64_t wide_tiles = static_cast<int64_t>((n * G + le::kPrefixCols - 1) / le::kPrefixCols) * cfg.kv_heads *
                                ((end - begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys);
     const bool small_f32 = cfg.kv_dtype == LE_F32 && wide_tiles <= kSmallF32;
@@ -229,14 +229,14 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   // the chain of a tile's steps, the others by their keys' bytes; a CU holds
   // two workgroups. So the wide ones are cut to one a CU, beside which the
   // narrow ones stream (256 rows behind 16384 keys, 32/8 heads x 128, and 64 to
-  // 1024 keys of their own: 178 us, with two a CU 212), or to two where the
-  // narrow ones are few (without own keys: 115 us, with one a CU 120). The
-  // narrow ones are cut to the places left (64 rows behind 4096 keys and 16 to
-  // 512 of their own, 14/2 heads x 64: 14.4 us, cut to two a CU 16.9), with an
-  // fp32 cache, whose products count here too, to one a CU (24 rows behind 1500
-  // keys 12.3 us, two a CU 16.7), but not where they fill the chip as they are,
-  // up to 1024 keys (48 sequences of 5 to 700 keys, 8 kv heads: 19.8 us, cut at
-  // 512 keys 21.9).
+  // 1024 keys of their own: 176 us, with two a CU 208), or to two where the
+  // narrow ones are few (122 rows after 131072 keys: 340 us, with one a CU 436).
+  // The narrow ones are cut to the places left (64 rows behind 4096 keys and 16
+  // to 512 of their own, 14/2 heads x 64: 12.9 us, to 64 keys each 15.7), with
+  // an fp32 cache, whose products count here too, to one a CU (24 rows behind
+  // 1500 keys 12.0 us, in parts twice as long 15.2), but not where they fill the
+  // chip as they are, up to 1024 keys (48 sequences of 5 to 700 keys, 8 kv
+  // heads: 19.6 us, cut at 512 keys 22.3).
   const int quantum = std::max(le::kPrefixTileKeys, bs);
   auto wide = [&](const Tile& t) { return static_cast<int>(t.rows.size()) * G > le::kPrefixNarrow; };
   std::vector<int64_t> len[2];

@@ -6,6 +6,10 @@ kernels behind a C ABI (include/llm_engine_amd.h).
     kernels.attention_decode(q, k_cache, v_cache, tables, table_offset, token_seq, token_pos, ...)
     plan = kernels.Plan(slices, q_heads, kv_heads, head_dim, block_size, kv_dtype).upload()
     kernels.ragged_paged_attention(q, k_cache, v_cache, plan, scale)
+    # sequences behind a shared prompt, with drafted tokens
+    prefix = kernels.PrefixPlan(slices, q_heads, kv_heads, head_dim, block_size, kv_dtype).upload()
+    kernels.shared_prefix_attention(q, k_cache, v_cache, prefix, scale)
+    kernels.verify_drafts(logits, cu_drafts, draft_tokens, accept_u, sample_u, max_drafts)
 """
 from ._lib import LIB_PATH, LeError, load  # noqa: F401
 
