@@ -316,7 +316,7 @@ typedef struct le_prefix_plan {
   int32_t n_parts;    /* partial results of split rows */
   int32_t rows_stride; /* rows and block ids listed for every item */
   int32_t ids_stride;
-  int32_t reserved_;
+  int32_t n_solo;     /* of the items, the last ones: a wave each, not a workgroup */
   int64_t saved_keys; /* cached rows that are not read again, summed over the groups */
   /* byte offsets inside the packed buffer */
   int64_t off_items, off_rows, off_item_ids, off_ids, off_part0, off_row_parts;

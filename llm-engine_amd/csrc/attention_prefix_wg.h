@@ -19,7 +19,8 @@
 //   * up to 32 columns, where three waves would idle: a wave has all columns
 //     and the 16 keys that it loads itself (16x16 MFMAs, no barrier), and the
 //     four waves' (m, l, o) are merged at the end. A single row is this case:
-//     it is bound by its keys' bytes, not by the products.
+//     it is bound by its keys' bytes, not by the products. Items of a few keys,
+//     where there are many, take a wave each, in the same way but for the merge.
 // S^T = K Q^T and O^T = V^T P^T: a lane holds one column, and its scores are
 // the second product's B operand as they are (A and B only have to agree on
 // the order of keys). q enters as it is and the scale is applied to the fp32
@@ -233,13 +234,14 @@ __device__ __forceinline__ int64_t record_of(const PrefixParams& p, const Prefix
 // a multiple of 16 on lie in one block, or in two of 8), so their addresses are
 // scalars and a lane adds its place in the rows. The block ids of 64 blocks at a
 // time wait in a register, a block a lane (first_id: the first ones, as listed).
-template <typename KV, int HD> struct Loader {
+template <typename KV, int HD, bool SOLO = false> struct Loader {
   using L = Geo<KV, HD>;
+  static constexpr int kStep = SOLO ? kKeys / kWaves : kKeys;  // keys of a tile
   const char* kbase;
   const char* vbase;
   const int32_t* ids;
   uint32_t row_bytes, block_bytes, num_blocks;  // a block is less than 4 GiB, the caller checks
-  int n_keys, wave, bs_shift, last_blk, window;
+  int n_keys, wave, row0, bs_shift, last_blk, window;  // row0: the wave's first row of a tile
   int32_t id_now, id_next;  // lane i: block 64 * window + i's id, and 64 further
   uint32_t off[L::IPW];
   struct Stage {  // a tile in flight
@@ -250,6 +252,7 @@ template <typename KV, int HD> struct Loader {
   __device__ __forceinline__ Loader(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int32_t first_id) {
     const int lane = threadIdx.x & (kWave - 1);
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    row0 = SOLO ? 0 : wave * 16;
     kbase = static_cast<const char*>(p.k_cache) + static_cast<int64_t>(kvh) * L::ROW;
     vbase = static_cast<const char*>(p.v_cache) + static_cast<int64_t>(kvh) * L::ROW;
     ids = p.ids + it.ids_off;
@@ -285,7 +288,7 @@ template <typename KV, int HD> struct Loader {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       // eight keys (past the range: its last eight again)
-      const int key = min(rel + wave * 16 + h * 8, (n_keys - 1) & ~7);
+      const int key = min(rel + row0 + h * 8, (n_keys - 1) & ~7);
       const int id = __builtin_amdgcn_readlane(id_now, (key >> bs_shift) & (kWave - 1));
       const bool in = static_cast<uint32_t>(id) < num_blocks;
       st.gone |= in ? 0u : 1u << h;
@@ -302,7 +305,7 @@ template <typename KV, int HD> struct Loader {
   // what the cache holds there need not be 0), and K and V rows without a block.
   __device__ __forceinline__ void stash(const Stage& st, char* buf, int rel) const {
     const int lane = threadIdx.x & (kWave - 1);
-    const int live = n_keys - (rel + wave * 16);
+    const int live = n_keys - (rel + row0);
     char* dst = buf + wave * L::IPW * 1024 + lane * 16;
 #pragma unroll
     for (int j = 0; j < L::IPW; j++) {
@@ -338,21 +341,22 @@ __device__ __forceinline__ void shared_tiles(Loader<KV, HD>& ld, typename Loader
 }
 // A wave's own rows: two tiles in flight beside the one in use (what bounds
 // such items is how many bytes are on their way), no barrier.
-template <typename KV, int HD, typename F>
-__device__ __forceinline__ void own_tiles(Loader<KV, HD>& ld, typename Loader<KV, HD>::Stage& a, Smem<KV, HD>& sm,
-                                          F tile) {
-  typename Loader<KV, HD>::Stage b;
-  const int n_tiles = (ld.n_keys + kKeys - 1) / kKeys;
-  if (n_tiles > 1) ld.issue(b, kKeys);
+template <typename KV, int HD, bool SOLO, typename F>
+__device__ __forceinline__ void own_tiles(Loader<KV, HD, SOLO>& ld, typename Loader<KV, HD, SOLO>::Stage& a,
+                                          Smem<KV, HD>& sm, F tile) {
+  constexpr int kStep = Loader<KV, HD, SOLO>::kStep;
+  typename Loader<KV, HD, SOLO>::Stage b;
+  const int n_tiles = (ld.n_keys + kStep - 1) / kStep;
+  if (n_tiles > 1) ld.issue(b, kStep);
   for (int t = 0; t < n_tiles; t += 2) {
-    const int rel = t * kKeys;
+    const int rel = t * kStep;
     ld.stash(a, sm.lds[0], rel);
-    if (t + 2 < n_tiles) ld.issue(a, rel + 2 * kKeys);
+    if (t + 2 < n_tiles) ld.issue(a, rel + 2 * kStep);
     tile(sm.lds[0], rel);
     if (t + 1 >= n_tiles) break;
-    ld.stash(b, sm.lds[1], rel + kKeys);
-    if (t + 3 < n_tiles) ld.issue(b, rel + 3 * kKeys);
-    tile(sm.lds[1], rel + kKeys);
+    ld.stash(b, sm.lds[1], rel + kStep);
+    if (t + 3 < n_tiles) ld.issue(b, rel + 3 * kStep);
+    tile(sm.lds[1], rel + kStep);
   }
 }
 
@@ -548,7 +552,8 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
 // NC column tiles of 16, known at compile time: with a branch around the second
 // tile's products the compiler left the first one's result a wait too short on
 // the way past the branch (fp32: a score without its last product).
-template <typename ACT, typename KV, int HD, int NC>
+// SOLO: the wave has the item for itself, all keys.
+template <typename ACT, typename KV, int HD, int NC, bool SOLO>
 __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int32_t first_id,
                                           Smem<KV, HD>& sm) {
   using X = operand<ACT, KV>;
@@ -558,9 +563,9 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
   const int lane = threadIdx.x & (kWave - 1);
   const int l16 = lane & 15, g = lane >> 4;
   const int G = p.q_heads / p.kv_heads;
-  Loader<KV, HD> ld(p, it, item, kvh, first_id);
+  Loader<KV, HD, SOLO> ld(p, it, item, kvh, first_id);
   const int wave = ld.wave;
-  typename Loader<KV, HD>::Stage first;
+  typename Loader<KV, HD, SOLO>::Stage first;
   ld.issue(first, 0);
   Column c[NC];
   typename M::frag qb[NC][KS];
@@ -570,7 +575,7 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qb[n][ks] = q_frag<ACT, X>(p, c[n], HD, ks * 32 + g * 8);
   }
-  if (wave == 0 && g == 0) {
+  if (!SOLO && wave == 0 && g == 0) {
 #pragma unroll
     for (int n = 0; n < NC; n++)
       if (c[n].ok) sm.row[(n * 16 + l16) / G] = make_int2(c[n].token, c[n].part0);
@@ -587,7 +592,7 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
   }
   const float scale = p.scale_log2;
   own_tiles(ld, first, sm, [&](const char* tile, int rel) {
-    const int key0 = rel + wave * 16;  // this wave's keys
+    const int key0 = rel + ld.row0;  // this wave's keys
     if (key0 >= ld.n_keys) return;
     const char* b = tile + wave * 16 * L::ROW;
     const char* bv = b + L::K_BYTES;
@@ -661,6 +666,29 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
     }
   });
 
+  if constexpr (SOLO) {
+    // acc[n][d][i] = O[column 16 n + l16][dim 16 d + 4 g + i]
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+      const float l = rows_sum(lsum[n]);
+      if (!c[n].ok) continue;
+      if (it.part < 0) {
+        ACT* out = static_cast<ACT*>(p.out) + (static_cast<int64_t>(c[n].token) * p.q_heads + c[n].head) * HD + g * 4;
+        const float inv = 1.f / l;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+          const float f[4] = {acc[n][d][0] * inv, acc[n][d][1] * inv, acc[n][d][2] * inv, acc[n][d][3] * inv};
+          elem<ACT>::store4(out + d * 16, f);
+        }
+      } else {
+        const int64_t rec = record_of(p, it, c[n].part0, c[n].head);
+#pragma unroll
+        for (int d = 0; d < DT; d++) *reinterpret_cast<f32x4*>(p.acc + rec * HD + d * 16 + g * 4) = acc[n][d];
+        if (g == 0) p.ml[rec] = make_float2(m[n], l);
+      }
+    }
+    return;
+  }
   // ---- the four waves' results, in the tiles' place: 16 columns at a time,
   // waves 0 and 1 in the first buffer, 2 and 3 in the second ----
   // acc[n][d][i] = O[column 16 n + l16][dim 16 d + 4 g + i]
@@ -710,17 +738,30 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
 }
 
 template <typename ACT, typename KV, int HD>
-__global__ __launch_bounds__(kThreads, (std::is_same_v<operand<ACT, KV>, float> ? 1 : 2)) void prefix_kernel(PrefixParams p) {
+__global__ __launch_bounds__(kThreads, (std::is_same_v<operand<ACT, KV>, float> && HD > 64 ? 1 : 2)) void prefix_kernel(PrefixParams p) {
   __shared__ Smem<KV, HD> sm;
   // an item's kv heads lie side by side: their rows are neighbours in the cache
-  const int item = blockIdx.x / p.kv_heads, kvh = blockIdx.x - item * p.kv_heads;
+  const uint32_t shared = static_cast<uint32_t>(p.n_items - p.n_solo) * p.kv_heads;
+  uint32_t unit = blockIdx.x;
+  if (unit >= shared) {  // an item a wave
+    unit = shared + (unit - shared) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (unit >= static_cast<uint32_t>(p.n_items) * p.kv_heads) return;
+  }
+  const int item = unit / p.kv_heads, kvh = unit - item * p.kv_heads;
   const int32_t first_id = p.item_ids[static_cast<int64_t>(item) * p.ids_stride +
                                       min(static_cast<int>(threadIdx.x & (kWave - 1)), p.ids_stride - 1)];
   const PrefixItem it = p.items[item];
   const int cols = it.n_rows * (p.q_heads / p.kv_heads);
-  if (cols <= 16) narrow_item<ACT, KV, HD, 1>(p, it, item, kvh, first_id, sm);
-  else if (cols <= kNarrow) narrow_item<ACT, KV, HD, 2>(p, it, item, kvh, first_id, sm);
-  else wide_item<ACT, KV, HD>(p, it, item, kvh, first_id, sm);
+  if (blockIdx.x >= shared) {
+    if (cols <= 16) narrow_item<ACT, KV, HD, 1, true>(p, it, item, kvh, first_id, sm);
+    else narrow_item<ACT, KV, HD, 2, true>(p, it, item, kvh, first_id, sm);
+  } else if (cols <= 16) {
+    narrow_item<ACT, KV, HD, 1, false>(p, it, item, kvh, first_id, sm);
+  } else if (cols <= kNarrow) {
+    narrow_item<ACT, KV, HD, 2, false>(p, it, item, kvh, first_id, sm);
+  } else {
+    wide_item<ACT, KV, HD>(p, it, item, kvh, first_id, sm);
+  }
 }
 
 // ---- rows of several parts: a wave for each (row, head) ----
@@ -785,7 +826,8 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(PrefixParams p) 
 
 template <typename ACT, typename KV, int HD>
 hipError_t launch_prefix(const PrefixParams& p, hipStream_t stream) {
-  prefix_kernel<ACT, KV, HD><<<static_cast<unsigned>(p.n_items) * static_cast<unsigned>(p.kv_heads), kThreads, 0, stream>>>(p);
+  const int64_t solo = static_cast<int64_t>(p.n_solo) * p.kv_heads, units = static_cast<int64_t>(p.n_items) * p.kv_heads;
+  prefix_kernel<ACT, KV, HD><<<static_cast<unsigned>(units - solo + (solo + kWaves - 1) / kWaves), kThreads, 0, stream>>>(p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.n_parts == 0) return e;
   const int64_t waves = static_cast<int64_t>(p.n_tokens) * p.q_heads;

@@ -138,7 +138,8 @@ struct PrefixParams {
   float* acc;                // [records][q_heads][head_dim] unnormalised
   float2* ml;                // [records][q_heads] (max in log2 units, sum)
   int rows_stride, ids_stride;
-  int n_items, n_tokens, n_parts, q_heads, kv_heads, head_dim, block_size;
+  int n_items, n_solo;       // items; the last ones, a wave each
+  int n_tokens, n_parts, q_heads, kv_heads, head_dim, block_size;
   float scale_log2;          // > 0
   int negate;                // the scale was negative: q changes its sign
   int64_t num_cache_blocks;

@@ -30,6 +30,8 @@ constexpr int kMinSharedKeys = 64;    // a shorter common beginning is not worth
 constexpr int kMaxParts = 128;        // partitions of a tile
 constexpr int kCus = 256;             // MI355X
 constexpr int kWideCost = 2;          // time of a wide tile's keys, in narrow ones
+constexpr int kSoloKeys = 32;         // keys of a narrow item up to which a wave takes it alone
+constexpr int kMinF32 = 4;            // LDS tiles of an fp32 item that is not narrow, at least
 constexpr int kSmallF32 = 256;        // LDS tiles of wide fp32 items up to which narrow ones take their place
 
 int64_t align256(int64_t x) { return (x + 255) & ~static_cast<int64_t>(255); }
@@ -237,7 +239,12 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   // 1500 keys 12.0 us, in parts twice as long 15.2), but not where they fill the
   // chip as they are, up to 1024 keys (48 sequences of 5 to 700 keys, 8 kv
   // heads: 19.6 us, cut at 512 keys 22.3).
+  // Wide fp32 tiles of head_dim 64, two a CU, hide each other's softmax (3 x 220
+  // rows behind 5200 keys, 12 heads: 131 us, one a CU 150), from 256 keys on (30
+  // rows behind 8192, 32/4 heads: 32 us, cut at 128 keys 37); of head_dim 128
+  // one fits.
   const int quantum = std::max(le::kPrefixTileKeys, bs);
+  const int64_t places = cfg.kv_dtype == LE_F32 && cfg.head_dim > 64 ? kCus : 2 * kCus;  // workgroups at once
   auto wide = [&](const Tile& t) { return static_cast<int>(t.rows.size()) * G > le::kPrefixNarrow; };
   std::vector<int64_t> len[2];
   int64_t work[2] = {0, 0};
@@ -246,11 +253,13 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
     work[wide(t)] += len[wide(t)].back();
   }
   int64_t part[2];
-  part[1] = part_tiles(len[1], cfg.kv_heads, work[0] * 8 < work[1] ? 2 * kCus : kCus);
+  const bool f32 = cfg.kv_dtype == LE_F32;
+  part[1] = part_tiles(len[1], cfg.kv_heads, work[0] * 8 < work[1] || (f32 && cfg.head_dim == 64) ? places : kCus);
+  if (f32) part[1] = std::max<int64_t>(part[1], kMinF32);
   int64_t wide_groups = 0;
   for (int64_t n : len[1]) wide_groups += (n + part[1] - 1) / part[1] * cfg.kv_heads;
   part[0] = part_tiles(len[0], cfg.kv_heads,
-                       cfg.kv_dtype == LE_F32 ? kCus : 2 * kCus - std::min<int64_t>(wide_groups, kCus));
+                       f32 ? kCus : 2 * kCus - std::min<int64_t>(wide_groups, kCus));
   if (static_cast<int64_t>(len[0].size()) * cfg.kv_heads >= kCus) part[0] = std::max<int64_t>(part[0], 16);
   for (int k = 0; k < 2; k++) {
     const int asked = k ? cfg.chunk_partition_tokens : cfg.partition_tokens;
@@ -300,6 +309,15 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   }
   auto cost = [&](const Placed& a) { return static_cast<int64_t>(a.item.key_end - a.item.key_begin) * (wide(*a.tile) ? kWideCost : 1); };
   std::stable_sort(items.begin(), items.end(), [&](const Placed& a, const Placed& b) { return cost(a) > cost(b); });
+  // Where there are more workgroups than places, an item of a few keys is given
+  // to one wave: alone it would keep four waves for the time of a few trips to
+  // memory (256 rows behind 512 keys and 1 to 30 of their own, 32/8 heads x 128:
+  // 24 us, 33 without; 234 rows behind 80 and 3, fp32, 32/4 x 64: 16, 21; where
+  // they all fit it is slower: 4 rows behind 512 keys and 8 to 100, 10.0 us
+  // against 7.9; items up to 64 keys: 4 x 32 rows 13.2 us, 12.7).
+  const bool full = n_items * cfg.kv_heads > places;
+  auto solo = [&](const Placed& a) { return full && !wide(*a.tile) && a.item.key_end - a.item.key_begin <= kSoloKeys; };
+  const auto first_solo = std::stable_partition(items.begin(), items.end(), [&](const Placed& a) { return !solo(a); });
 
   // ---- layout and copy ----
   le_prefix_plan out{};
@@ -317,6 +335,7 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   };
   out.rows_stride = rows_stride;
   out.ids_stride = ids_stride;
+  out.n_solo = static_cast<int32_t>(items.end() - first_solo);
   const size_t n = items.size();
   place(out.off_items, n * sizeof(PrefixItem));
   place(out.off_rows, n * rows_stride * sizeof(PrefixRow));

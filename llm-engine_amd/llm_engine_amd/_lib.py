@@ -98,7 +98,7 @@ class PrefixStepPlan(ctypes.Structure):
         ("n_parts", ctypes.c_int32),
         ("rows_stride", ctypes.c_int32),
         ("ids_stride", ctypes.c_int32),
-        ("reserved_", ctypes.c_int32),
+        ("n_solo", ctypes.c_int32),
         ("saved_keys", ctypes.c_int64),
         ("off_items", ctypes.c_int64),
         ("off_rows", ctypes.c_int64),

@@ -228,6 +228,17 @@ def test_nan_and_infinities_stay_with_their_rows(gpu, kv):
     assert torch.equal(got[~(bad | drop)], clean[~(bad | drop)])
 
 
+@pytest.mark.parametrize("heads,n", [(LLAMA, 141), (WIDE, 75), ((3, 3, 128), 181), ((40, 5, 64), 109)])
+@pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("bf16", "f32")])
+def test_many_short_sequences(gpu, heads, n, act, kv):
+    """More workgroups than the chip holds: items of up to 32 keys take a wave
+    each; drafts, keys from one on, and rows with nothing shared among them."""
+    seqs = [(0, 12, 1 + i % 45, 1 + min(i % 45, i % 4)) for i in range(n)] + [(1 + i, 0, 1 + i, 1) for i in range(7)]
+    s = Step(seqs, heads, act=act, kv=kv, seed=24)
+    assert 0 < s.plan.plan.n_solo < s.plan.plan.n_items
+    s.check()
+
+
 @pytest.mark.parametrize("kv", ["bf16", "f16", "f32"])
 def test_dead_cache_rows_are_not_read(gpu, kv):
     """NaN in every cache row that no sequence has computed (the rest of the last

@@ -194,6 +194,18 @@ def test_random_steps_in_asked_tiles(seed):
     assert (arrays(plan)[0][:, 0] * (heads[0] // heads[1]) <= tile).all()
 
 
+@pytest.mark.parametrize("n,heads,kv,solo", [(40, (32, 4, 64), torch.bfloat16, False), (150, (32, 4, 64), torch.bfloat16, True),
+                                             (40, (32, 8, 128), torch.float32, True), (40, (32, 8, 128), torch.bfloat16, False)])
+def test_short_items_of_a_full_step_take_a_wave(n, heads, kv, solo):
+    """The last items of the list, of at most 32 keys and columns."""
+    seqs = [(np.concatenate([np.arange(20), 100 + 5 * i + np.arange(5)]), 320 + i % 70, 1 + i % 3) for i in range(n)]
+    plan = check(seqs, heads, kv=kv)
+    items, P = arrays(plan)[0], plan.plan
+    assert (P.n_solo > 0) == solo
+    short = (items[:, 3] - items[:, 2] <= 32) & (items[:, 0] * (heads[0] // heads[1]) <= 32)
+    assert P.n_solo == (int(short.sum()) if solo else 0) and short[P.n_items - P.n_solo:].all()
+
+
 def test_attention_refusals_without_launch():
     plan = pack([(np.arange(30), 400, 1), (np.arange(30), 410, 1)])
     P, L = plan.plan, _lib.load()
