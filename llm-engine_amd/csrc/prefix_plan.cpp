@@ -30,6 +30,7 @@ constexpr int kMinSharedKeys = 64;    // a shorter common beginning is not worth
 constexpr int kMaxParts = 128;        // partitions of a tile
 constexpr int kCus = 256;             // MI355X
 constexpr int kWideCost = 2;          // time of a wide tile's keys, in narrow ones
+constexpr int kShortOwn = 256;        // keys of a sequence that few columns attend in narrow tiles
 constexpr int kSoloKeys = 32;         // keys of a narrow item up to which a wave takes it alone
 constexpr int kMinF32 = 4;            // LDS tiles of an fp32 item that is not narrow, at least
 constexpr int kSmallF32 = 256;        // LDS tiles of wide fp32 items up to which narrow ones take their place
@@ -192,7 +193,12 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
     const int64_t wide_tiles = static_cast<int64_t>((n * G + le::kPrefixCols - 1) / le::kPrefixCols) * cfg.kv_heads *
                                ((end - begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys);
     const bool small_f32 = cfg.kv_dtype == LE_F32 && wide_tiles <= kSmallF32;
-    const int tile_rows = (cfg.chunk_q_tile > 0 ? cfg.chunk_q_tile : small_f32 ? le::kPrefixNarrow : le::kPrefixCols) / G;
+    // A sequence's 33 to 64 columns would leave half of a wide tile's waves
+    // idle: over a few keys two narrow tiles are quicker (48 sequences of up to
+    // 8 rows behind 2000 keys, 28/4 heads x 128, own keys 8 to 700: 31 us, 35
+    // as wide ones; up to 1024 keys narrow, 33).
+    const bool few = causal && n * G <= 2 * le::kPrefixNarrow && end - begin <= kShortOwn;
+    const int tile_rows = (cfg.chunk_q_tile > 0 ? cfg.chunk_q_tile : small_f32 || few ? le::kPrefixNarrow : le::kPrefixCols) / G;
     const int count = (n + tile_rows - 1) / tile_rows;
     for (int k = 0; k < count; k++) {
       const int a = static_cast<int>(static_cast<int64_t>(k) * n / count);
