@@ -32,6 +32,7 @@ constexpr int kCus = 256;             // MI355X
 constexpr int kWideCost = 2;          // time of a wide tile's keys, in narrow ones
 constexpr int kShortOwn = 256;        // keys of a sequence that few columns attend in narrow tiles
 constexpr int kSoloKeys = 32;         // keys of a narrow item up to which a wave takes it alone
+constexpr int kExtra = 6;             // time of a 16-bit workgroup around its tiles, in LDS tiles
 constexpr int kMinF32 = 4;            // LDS tiles of an fp32 item that is not narrow, at least
 constexpr int kSmallF32 = 256;        // LDS tiles of wide fp32 items up to which narrow ones take their place
 
@@ -118,6 +119,30 @@ int64_t part_tiles(const std::vector<int64_t>& len, int kv_heads, int64_t slots)
     if (n <= slots) break;
   }
   return std::min(t, most);
+}
+
+// The same of tiles whose products count: the partition with which the rounds of
+// `slots` workgroups, each as long as a partition and the time of `extra` LDS
+// tiles around it, end first. (2 x 315 rows behind 10624 keys, 32/4 heads x 64:
+// 104 us in three rounds, 162 in one that fills 160 of 256 places.)
+int64_t round_tiles(const std::vector<int64_t>& len, int kv_heads, int64_t slots, int64_t extra) {
+  int64_t work = 0, most = 1;
+  for (int64_t n : len) {
+    work += n * kv_heads;
+    most = std::max(most, n);
+  }
+  int64_t best = most, least = INT64_MAX;
+  for (int64_t t = std::max<int64_t>(1, work / (8 * slots));; t += std::max<int64_t>(1, t / 16)) {
+    t = std::min(t, most);
+    int64_t n = 0;
+    for (int64_t x : len) n += (x + t - 1) / t * kv_heads;
+    const int64_t time = (n + slots - 1) / slots * (t + extra);
+    if (time <= least) {
+      least = time;
+      best = t;
+    }
+    if (t == most) return best;
+  }
 }
 
 struct Tile {
@@ -252,23 +277,35 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   const int quantum = std::max(le::kPrefixTileKeys, bs);
   const int64_t places = cfg.kv_dtype == LE_F32 && cfg.head_dim > 64 ? kCus : 2 * kCus;  // workgroups at once
   auto wide = [&](const Tile& t) { return static_cast<int>(t.rows.size()) * G > le::kPrefixNarrow; };
-  std::vector<int64_t> len[2];
-  int64_t work[2] = {0, 0};
+  // Narrow tiles of shared keys (kind 2) are few and long beside the sequences'
+  // own ones, and cut apart from them (4 x 10 sequences of up to 4 rows behind
+  // 1184 keys and 3 of their own, 12 heads x 64: 13 us, together 24).
+  auto kind = [&](const Tile& t) { return wide(t) ? 1 : t.causal ? 0 : 2; };
+  std::vector<int64_t> len[3];
+  int64_t work[3] = {0, 0, 0};
   for (const Tile& t : tiles) {
-    len[wide(t)].push_back((t.key_end - t.key_begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys);
-    work[wide(t)] += len[wide(t)].back();
+    len[kind(t)].push_back((t.key_end - t.key_begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys);
+    work[kind(t)] += len[kind(t)].back();
   }
-  int64_t part[2];
   const bool f32 = cfg.kv_dtype == LE_F32;
-  part[1] = part_tiles(len[1], cfg.kv_heads, work[0] * 8 < work[1] || (f32 && cfg.head_dim == 64) ? places : kCus);
+  int64_t part[3];
+  auto workgroups = [&](int k) {
+    int64_t n = 0;
+    for (int64_t x : len[k]) n += (x + part[k] - 1) / part[k] * cfg.kv_heads;
+    return n;
+  };
+  part[1] = round_tiles(len[1], cfg.kv_heads,
+                        (work[0] + work[2]) * 8 < work[1] || (f32 && cfg.head_dim == 64) ? places : kCus,
+                        f32 ? kExtra / 2 : kExtra);
   if (f32) part[1] = std::max<int64_t>(part[1], kMinF32);
-  int64_t wide_groups = 0;
-  for (int64_t n : len[1]) wide_groups += (n + part[1] - 1) / part[1] * cfg.kv_heads;
-  part[0] = part_tiles(len[0], cfg.kv_heads,
-                       f32 ? kCus : 2 * kCus - std::min<int64_t>(wide_groups, kCus));
-  if (static_cast<int64_t>(len[0].size()) * cfg.kv_heads >= kCus) part[0] = std::max<int64_t>(part[0], 16);
-  for (int k = 0; k < 2; k++) {
-    const int asked = k ? cfg.chunk_partition_tokens : cfg.partition_tokens;
+  const int64_t own = static_cast<int64_t>(len[0].size()) * cfg.kv_heads;
+  const int64_t left = f32 ? kCus - std::min<int64_t>(workgroups(1), kCus / 2)
+                           : 2 * kCus - std::min<int64_t>(workgroups(1), kCus);
+  part[2] = part_tiles(len[2], cfg.kv_heads, std::max(left - own, left / 2));
+  part[0] = part_tiles(len[0], cfg.kv_heads, std::max<int64_t>(left - workgroups(2), 1));
+  if (own >= kCus) part[0] = std::max<int64_t>(part[0], 16);
+  for (int k = 0; k < 3; k++) {
+    const int asked = k == 1 ? cfg.chunk_partition_tokens : cfg.partition_tokens;
     part[k] = asked > 0 ? asked : part[k] * le::kPrefixTileKeys;
     part[k] = (part[k] + quantum - 1) / quantum * quantum;
   }
@@ -276,7 +313,7 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   int64_t n_items = 0;
   for (Tile& t : tiles) {
     const int64_t units = (t.key_end - t.key_begin + quantum - 1) / quantum;
-    t.parts = static_cast<int>(std::min<int64_t>(kMaxParts, (units * quantum + part[wide(t)] - 1) / part[wide(t)]));
+    t.parts = static_cast<int>(std::min<int64_t>(kMaxParts, (units * quantum + part[kind(t)] - 1) / part[kind(t)]));
     t.part_first = n_parts[t.rows[0]];
     for (int32_t r : t.rows) n_parts[r] += t.parts;
     n_items += t.parts;
