@@ -63,10 +63,16 @@ def _f32(t: torch.Tensor, n: int, device: int) -> bool:
     return t.get_device() == device and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements from row to row of a 2-d tensor; a single row's is its length
-    (whatever its stride says), rounded up to whole 16-byte pieces of any type."""
-    return t.stride(0) if t.size(0) > 1 else (t.size(1) + 7) // 8 * 8
+def _rows(t: torch.Tensor) -> tuple[int, int, int]:
+    """(rows, columns, elements from row to row) of a 2-d tensor with unit column
+    stride, or (-1, -1, -1); a single row's step is its length (whatever its
+    stride says), rounded up to whole 16-byte pieces of any type."""
+    if t.dim() != 2:
+        return -1, -1, -1
+    (n, columns), (step, unit) = t.shape, t.stride()
+    if unit != 1:
+        return -1, -1, -1
+    return n, columns, step if n > 1 else (columns + 7) // 8 * 8
 
 
 def _bytes(t: torch.Tensor | None) -> int:
@@ -159,19 +165,21 @@ def qk_norm_rope_store_kv(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
     after the bias, in fp32 with one rounding per stored value. Returns q:
     [N, q_heads*head_dim]."""
     dev = qkv.get_device()
-    if dev < 0 or qkv.dim() != 2 or qkv.stride(1) != 1:
+    n, width, step = _rows(qkv)
+    if dev < 0 or n < 0:
         raise ValueError("qkv: cuda [N, row] with unit column stride")
-    n, row, kv_dim, half = qkv.size(0), (q_heads + 2 * kv_heads) * head_dim, kv_heads * head_dim, head_dim // 2
-    if qkv.size(1) < row:
+    row, kv_dim, half = (q_heads + 2 * kv_heads) * head_dim, kv_heads * head_dim, head_dim // 2
+    if width < row:
         raise ValueError("qkv rows too short")
-    max_pos = cos_t.size(0)
-    if cos_t.shape != sin_t.shape or not (_f32(cos_t, max_pos * half, dev) and _f32(sin_t, max_pos * half, dev)):
+    table = cos_t.shape
+    max_pos = table[0]
+    if table != sin_t.shape or not (_f32(cos_t, max_pos * half, dev) and _f32(sin_t, max_pos * half, dev)):
         raise ValueError("cos_t, sin_t: contiguous fp32 cuda [max_pos, head_dim/2]")
     if not (_f32(q_norm, head_dim, dev) and _f32(k_norm, head_dim, dev)):
         raise ValueError("q_norm, k_norm: contiguous fp32 cuda [head_dim]")
-    num_slots = k_cache.size(0)
+    num_slots = k_cache.shape[0]
     if not (k_cache.dtype == v_cache.dtype and k_cache.numel() == v_cache.numel() == num_slots * kv_dim
-            and v_cache.size(0) == num_slots and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and v_cache.shape[0] == num_slots and k_cache.is_contiguous() and v_cache.is_contiguous()
             and k_cache.get_device() == v_cache.get_device() == dev):
         raise ValueError("k_cache, v_cache: contiguous cuda [num_slots, kv_heads*head_dim], alike")
     if not (_i32(positions, n, dev) and _i32(slots, n, dev)):
@@ -183,7 +191,7 @@ def qk_norm_rope_store_kv(qkv: torch.Tensor, positions: torch.Tensor, slots: tor
     elif not (q_out.is_contiguous() and q_out.dtype == qkv.dtype and q_out.numel() == n * q_heads * head_dim
               and q_out.get_device() == dev):
         raise ValueError("q_out: contiguous cuda [N, q_heads*head_dim] in qkv's dtype")
-    _launch("le_qk_norm_rope_kv_cache_write", dev, stream, qkv.data_ptr(), _dt(qkv), _row_stride(qkv),
+    _launch("le_qk_norm_rope_kv_cache_write", dev, stream, qkv.data_ptr(), _dt(qkv), step,
             None if bias is None else bias.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), eps, positions.data_ptr(),
             slots.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), max_pos, n, q_heads, kv_heads, head_dim,
             q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _dt(k_cache), num_slots)
@@ -218,10 +226,10 @@ def verify_drafts(logits: torch.Tensor, cu_drafts: torch.Tensor, draft_tokens: t
     the number accepted [sequences] int32)."""
     dev = logits.get_device()
     n_drafts, n_seqs = draft_tokens.numel(), cu_drafts.numel() - 1
-    if dev < 0 or logits.dim() != 2 or logits.stride(1) != 1:
+    rows, vocab, step = _rows(logits)
+    if dev < 0 or rows < 0:
         raise ValueError("logits: cuda [rows, vocab] with unit column stride")
-    vocab = logits.size(1)
-    if n_seqs < 0 or logits.size(0) != n_drafts + n_seqs:
+    if n_seqs < 0 or rows != n_drafts + n_seqs:
         raise ValueError("logits: one row per draft and one per sequence")
     if not (_i32(cu_drafts, n_seqs + 1, dev) and _i32(draft_tokens, n_drafts, dev)):
         raise ValueError("cu_drafts, draft_tokens: contiguous int32 cuda")
@@ -229,10 +237,12 @@ def verify_drafts(logits: torch.Tensor, cu_drafts: torch.Tensor, draft_tokens: t
         raise ValueError("accept_u, sample_u: contiguous fp32 cuda, one per draft and one per sequence")
     if temperature is not None and not _f32(temperature, n_seqs, dev):
         raise ValueError("temperature: contiguous fp32 cuda, one per sequence")
-    if draft_probs is not None and not (draft_probs.dim() == 2 and draft_probs.size(0) == n_drafts
-                                        and draft_probs.size(1) == vocab and draft_probs.stride(1) == 1
-                                        and draft_probs.get_device() == dev):
-        raise ValueError("draft_probs: cuda [drafts, vocab] with unit column stride")
+    probs = probs_dtype = probs_step = 0
+    if draft_probs is not None:
+        probs_rows, probs_columns, probs_step = _rows(draft_probs)
+        if probs_rows != n_drafts or probs_columns != vocab or draft_probs.get_device() != dev:
+            raise ValueError("draft_probs: cuda [drafts, vocab] with unit column stride")
+        probs, probs_dtype = draft_probs.data_ptr(), _dt(draft_probs)
     if out is None:
         out = _empty(stream, (n_seqs, max_drafts + 1), torch.int32, logits.device)
     elif not (_i32(out, 0, dev) and out.dim() == 2 and out.size(0) == n_seqs and out.size(1) == max_drafts + 1):
@@ -246,12 +256,10 @@ def verify_drafts(logits: torch.Tensor, cu_drafts: torch.Tensor, draft_tokens: t
         workspace = _empty(stream, (need,), torch.uint8, logits.device)
     elif workspace is not None and workspace.get_device() != dev:
         raise ValueError("workspace: on the tensors' device")
-    _launch("le_verify_drafts", dev, stream, logits.data_ptr(), _dt(logits), _row_stride(logits), vocab,
-            None if draft_probs is None else draft_probs.data_ptr(), 0 if draft_probs is None else _dt(draft_probs),
-            0 if draft_probs is None else _row_stride(draft_probs), cu_drafts.data_ptr(), draft_tokens.data_ptr(),
-            accept_u.data_ptr(), sample_u.data_ptr(), None if temperature is None else temperature.data_ptr(), n_seqs,
-            n_drafts, max_drafts, out.data_ptr(), n_accepted.data_ptr(),
-            None if workspace is None else workspace.data_ptr(), _bytes(workspace))
+    _launch("le_verify_drafts", dev, stream, logits.data_ptr(), _dt(logits), step, vocab, probs, probs_dtype,
+            probs_step, cu_drafts.data_ptr(), draft_tokens.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(),
+            None if temperature is None else temperature.data_ptr(), n_seqs, n_drafts, max_drafts, out.data_ptr(),
+            n_accepted.data_ptr(), None if workspace is None else workspace.data_ptr(), _bytes(workspace))
     return out, n_accepted
 
 
