@@ -152,3 +152,34 @@ def test_upload_through_the_abi(gpu):
     assert _lib.load().le_prefix_plan_upload(ctypes.byref(plan.plan), plan.host.data_ptr(), buf.data_ptr(), raw) == 0
     plan.device_buf = buf
     assert torch.equal(kernels.shared_prefix_attention(s.q, s.k, s.v, plan, s.scale), want)
+
+
+def test_empty_steps(gpu):
+    """No rows, no sequences: nothing is launched, nothing changes."""
+    from llm_engine_amd import kernels
+    f = Flow(BATCH, QWEN, seed=8)
+    c, k = f.norm, f.step.k.clone()
+    q = kernels.qk_norm_rope_store_kv(c.qkv[:0], c.pos, c.slots, c.cos, c.sin, c.qw, c.kw, c.eps, *QWEN, c.k, c.v)
+    plan = kernels.PrefixPlan([], *QWEN, 16, torch.bfloat16).upload()
+    out = kernels.shared_prefix_attention(q, f.step.k, f.step.v, plan, 1.0)
+    none = torch.zeros(0, device=f.step.dev)
+    tokens, n = kernels.verify_drafts(torch.zeros(0, 50, device=f.step.dev), f.cu_dev[:1], f.tokens[:0], none, none, 3)
+    assert q.shape == out.shape == (0, 14 * 64) and tokens.shape == (0, 4) and n.shape == (0,)
+    torch.cuda.synchronize()
+    assert torch.equal(f.step.k, k)
+
+
+def test_two_steps_at_once(gpu):
+    """Two steps, each on a stream of its own, not waiting for each other: each
+    gives what it gives alone."""
+    flows = [Flow(SEQS, QWEN, seed=9), Flow([(0, 30, 20 + i % 30, 1 + i % 2) for i in range(90)], LLAMA, seed=10)]
+    want = [[t.clone() for t in f.run()] for f in flows]
+    streams = [torch.cuda.Stream() for _ in flows]
+    torch.cuda.synchronize()
+    got = [[] for _ in flows]
+    for _ in range(6):
+        for f, s, g in zip(flows, streams, got):
+            g.append(f.run(stream=s))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for r in g for a, b in zip(r, w))
