@@ -214,8 +214,16 @@ __device__ __forceinline__ Column column_of(const PrefixParams& p, const PrefixI
 // eight elements of a column's q from dim d on, with the scale's sign
 template <typename ACT, typename X>
 __device__ __forceinline__ typename mm<X>::frag q_frag(const PrefixParams& p, const Column& c, int hd, int d) {
+  const ACT* q = static_cast<const ACT*>(p.q) + (static_cast<int64_t>(c.token) * p.q_heads + c.head) * hd + d;
+  if constexpr (sizeof(X) == 2) {  // the same type: bits
+    u32x4 raw = *reinterpret_cast<const u32x4*>(q);
+    const uint32_t sign = p.negate ? 0x80008000u : 0u, keep = c.ok ? ~0u : 0u;
+#pragma unroll
+    for (int e = 0; e < 4; e++) raw[e] = (raw[e] ^ sign) & keep;
+    return __builtin_bit_cast(typename mm<X>::frag, raw);
+  }
   float f[8];
-  elem<ACT>::load8(static_cast<const ACT*>(p.q) + (static_cast<int64_t>(c.token) * p.q_heads + c.head) * hd + d, f);
+  elem<ACT>::load8(q, f);
   typename mm<X>::frag r;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
