@@ -231,6 +231,7 @@ int le_shared_prefix_attention(const void* q, le_dtype act_dtype, const void* k_
                                      align256(static_cast<size_t>(plan->n_parts) * cfg.q_heads * cfg.head_dim * sizeof(float)));
   }
   p.n_items = plan->n_items; p.n_solo = plan->n_solo; p.n_tokens = plan->n_tokens; p.n_parts = plan->n_parts;
+  p.per_row = 65536 / (cfg.q_heads / cfg.kv_heads) + 1;
   p.q_heads = cfg.q_heads; p.kv_heads = cfg.kv_heads; p.head_dim = cfg.head_dim; p.block_size = cfg.block_size;
   // the kernel's running maximum wants a positive factor; one of 0 becomes so
   // small that every score is 0 (and a masked one stays -inf)

@@ -198,10 +198,15 @@ struct Column {
   int token, part0, head, lim;
   bool ok;  // the column exists
 };
-__device__ __forceinline__ Column column_of(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int c) {
+// A column's row among its item's: c / G (c < 128, G <= 8: exact).
+__device__ __forceinline__ int row_index(const PrefixParams& p, int c) { return (c * p.per_row) >> 16; }
+// The item's row of a column (past its last: the list repeats that one).
+__device__ __forceinline__ PrefixRow row_of(const PrefixParams& p, int item, int c) {
+  return p.rows[static_cast<int64_t>(item) * p.rows_stride + min(row_index(p, c), p.rows_stride - 1)];
+}
+__device__ __forceinline__ Column column_of(const PrefixParams& p, const PrefixItem& it, const PrefixRow& row, int kvh, int c) {
   const int G = p.q_heads / p.kv_heads;
-  const int r = c / G;
-  const PrefixRow row = p.rows[static_cast<int64_t>(item) * p.rows_stride + min(r, p.rows_stride - 1)];
+  const int r = row_index(p, c);
   Column o;
   o.ok = r < it.n_rows;
   o.token = row.token;
@@ -257,7 +262,7 @@ template <typename KV, int HD, bool SOLO = false> struct Loader {
     uint32_t gone;  // bits 0 and 1: its rows 0-7 and 8-15 have no block
   };
 
-  __device__ __forceinline__ Loader(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int32_t first_id) {
+  __device__ __forceinline__ Loader(const PrefixParams& p, const PrefixItem& it, int kvh, int32_t first_id) {
     const int lane = threadIdx.x & (kWave - 1);
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     row0 = SOLO ? 0 : wave * 16;
@@ -370,25 +375,24 @@ __device__ __forceinline__ void own_tiles(Loader<KV, HD, SOLO>& ld, typename Loa
 
 // ---- more than 32 columns: 32 a wave ----
 template <typename ACT, typename KV, int HD>
-__device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int32_t first_id,
-                                          Smem<KV, HD>& sm) {
+__device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixItem& it, const PrefixRow& row, int kvh,
+                                          int32_t first_id, Smem<KV, HD>& sm) {
   using X = operand<ACT, KV>;
   using M = mm<X>;
   using L = Geo<KV, HD>;
   constexpr int KS = HD / 16, DT = HD / 32, U = kKeys / 32;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const int col = lane & 31, half = lane >> 5, l16 = lane & 15;
-  Loader<KV, HD> ld(p, it, item, kvh, first_id);
+  Loader<KV, HD> ld(p, it, kvh, first_id);
   typename Loader<KV, HD>::Stage first;
   ld.issue(first, 0);
-  const Column c = column_of(p, it, item, kvh, wave * 32 + col);
+  const Column c = column_of(p, it, row, kvh, wave * 32 + col);
   typename M::frag qb[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) qb[ks] = q_frag<ACT, X>(p, c, HD, ks * 16 + half * 8);
   // the wave's keys: none past the last one that any of its columns sees, and
   // no mask up to the first that one does not (columns without a row aside)
-  const int G = p.q_heads / p.kv_heads;
-  const bool any = wave * 32 / G < it.n_rows;
+  const bool any = row_index(p, wave * 32) < it.n_rows;
   int wave_lim = c.lim, free_lim = c.ok ? c.lim : INT32_MAX;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -562,8 +566,8 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
 // the way past the branch (fp32: a score without its last product).
 // SOLO: the wave has the item for itself, all keys.
 template <typename ACT, typename KV, int HD, int NC, bool SOLO>
-__device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixItem& it, int item, int kvh, int32_t first_id,
-                                          Smem<KV, HD>& sm) {
+__device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixItem& it, const PrefixRow* rows, int kvh,
+                                            int32_t first_id, Smem<KV, HD>& sm) {
   using X = operand<ACT, KV>;
   using M = mm<X>;
   using L = Geo<KV, HD>;
@@ -571,7 +575,7 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
   const int lane = threadIdx.x & (kWave - 1);
   const int l16 = lane & 15, g = lane >> 4;
   const int G = p.q_heads / p.kv_heads;
-  Loader<KV, HD, SOLO> ld(p, it, item, kvh, first_id);
+  Loader<KV, HD, SOLO> ld(p, it, kvh, first_id);
   const int wave = ld.wave;
   typename Loader<KV, HD, SOLO>::Stage first;
   ld.issue(first, 0);
@@ -579,14 +583,14 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
   typename M::frag qb[NC][KS];
 #pragma unroll
   for (int n = 0; n < NC; n++) {
-    c[n] = column_of(p, it, item, kvh, n * 16 + l16);
+    c[n] = column_of(p, it, rows[n], kvh, n * 16 + l16);
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) qb[n][ks] = q_frag<ACT, X>(p, c[n], HD, ks * 32 + g * 8);
   }
   if (!SOLO && wave == 0 && g == 0) {
 #pragma unroll
     for (int n = 0; n < NC; n++)
-      if (c[n].ok) sm.row[(n * 16 + l16) / G] = make_int2(c[n].token, c[n].part0);
+      if (c[n].ok) sm.row[row_index(p, n * 16 + l16)] = make_int2(c[n].token, c[n].part0);
   }
 
   f32x4 acc[NC][DT];
@@ -717,7 +721,7 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
     const int cols = min(16, it.n_rows * G - n * 16);
     for (int i = threadIdx.x; i < cols * PIECES; i += kThreads) {
       const int cl = i / PIECES, cc = n * 16 + cl, d = (i - cl * PIECES) * 4;
-      const int row = cc / G, head = kvh * G + cc - row * G;
+      const int row = row_index(p, cc), head = kvh * G + cc - row * G;
       const int2 o = sm.row[row];
       float M4 = -FLT_MAX;
 #pragma unroll
@@ -756,19 +760,23 @@ __global__ __launch_bounds__(kThreads, (std::is_same_v<operand<ACT, KV>, float> 
     if (unit >= static_cast<uint32_t>(p.n_items) * p.kv_heads) return;
   }
   const int item = unit / p.kv_heads, kvh = unit - item * p.kv_heads;
+  const int lane = threadIdx.x & (kWave - 1);
   const int32_t first_id = p.item_ids[static_cast<int64_t>(item) * p.ids_stride +
-                                      min(static_cast<int>(threadIdx.x & (kWave - 1)), p.ids_stride - 1)];
+                                      min(lane, p.ids_stride - 1)];
+  // the rows of a lane's columns, of every kind of tile: asked for beside the item
+  const PrefixRow wide_row = row_of(p, item, threadIdx.x / kWave * 32 + (lane & 31));
+  const PrefixRow rows[2] = {row_of(p, item, lane & 15), row_of(p, item, 16 + (lane & 15))};
   const PrefixItem it = p.items[item];
   const int cols = it.n_rows * (p.q_heads / p.kv_heads);
   if (blockIdx.x >= shared) {
-    if (cols <= 16) narrow_item<ACT, KV, HD, 1, true>(p, it, item, kvh, first_id, sm);
-    else narrow_item<ACT, KV, HD, 2, true>(p, it, item, kvh, first_id, sm);
+    if (cols <= 16) narrow_item<ACT, KV, HD, 1, true>(p, it, rows, kvh, first_id, sm);
+    else narrow_item<ACT, KV, HD, 2, true>(p, it, rows, kvh, first_id, sm);
   } else if (cols <= 16) {
-    narrow_item<ACT, KV, HD, 1, false>(p, it, item, kvh, first_id, sm);
+    narrow_item<ACT, KV, HD, 1, false>(p, it, rows, kvh, first_id, sm);
   } else if (cols <= kNarrow) {
-    narrow_item<ACT, KV, HD, 2, false>(p, it, item, kvh, first_id, sm);
+    narrow_item<ACT, KV, HD, 2, false>(p, it, rows, kvh, first_id, sm);
   } else {
-    wide_item<ACT, KV, HD>(p, it, item, kvh, first_id, sm);
+    wide_item<ACT, KV, HD>(p, it, wide_row, kvh, first_id, sm);
   }
 }
 

@@ -140,6 +140,7 @@ struct PrefixParams {
   int rows_stride, ids_stride;
   int n_items, n_solo;       // items; the last ones, a wave each
   int n_tokens, n_parts, q_heads, kv_heads, head_dim, block_size;
+  int per_row;               // 65536 / (q_heads / kv_heads) + 1
   float scale_log2;          // > 0
   int negate;                // the scale was negative: q changes its sign
   int64_t num_cache_blocks;
