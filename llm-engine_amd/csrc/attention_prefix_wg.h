@@ -33,10 +33,10 @@
 // uses the fp32 MFMA on widened operands.
 //
 // What bounds it: narrow tiles, HBM (256 sequences of 64 to 1024 keys, 8 kv
-// heads x 128, bf16: 109 us, 5.3 TB/s of K and V); wide ones, the products and
+// heads x 128, bf16: 108 us, 5.4 TB/s of K and V); wide ones, the products and
 // the softmax beside them, at the clock that they leave (122 rows after 131072
-// keys, 32/8 heads x 128: 340 us, 770 TFLOP/s; on zeros 267); small steps, the
-// chain of two launches (block ids, q, keys, record, merge: 8 us at least).
+// keys, 32/8 heads x 128: 327 us, 800 TFLOP/s; on zeros 264); small steps, the
+// chain of two launches (block ids, q, keys, record, merge: 7 us at least).
 #include <float.h>
 
 #include <type_traits>

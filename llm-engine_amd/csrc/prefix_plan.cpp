@@ -124,7 +124,7 @@ int64_t part_tiles(const std::vector<int64_t>& len, int kv_heads, int64_t slots)
 // The same of tiles whose products count: the partition with which the rounds of
 // `slots` workgroups, each as long as a partition and the time of `extra` LDS
 // tiles around it, end first. (2 x 315 rows behind 10624 keys, 32/4 heads x 64:
-// 104 us in three rounds, 162 in one that fills 160 of 256 places.)
+// 100 us in three rounds, 164 in one that fills 160 of 256 places.)
 int64_t round_tiles(const std::vector<int64_t>& len, int kv_heads, int64_t slots, int64_t extra) {
   int64_t work = 0, most = 1;
   for (int64_t n : len) {
@@ -213,8 +213,8 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
     const int n = static_cast<int>(rows.size());
     // fp32 products take 3.6 us per 64 keys (head_dim 64) in a wide tile and
     // 0.9 in a narrow one: a step too small to fill the chip with wide ones is
-    // cut into narrow ones (24 rows behind 1500 keys, 14/2 heads x 64: 12.0 us
-    // against 13.4; 128 rows behind 4096: 116 against 36).
+    // cut into narrow ones (24 rows behind 1500 keys, 14/2 heads x 64: 11.3 us
+    // against 25; 128 rows behind 4096: 59 against 31).
     const int64_t wide_tiles = static_cast<int64_t>((n * G + le::kPrefixCols - 1) / le::kPrefixCols) * cfg.kv_heads *
                                ((end - begin + le::kPrefixTileKeys - 1) / le::kPrefixTileKeys);
     const bool small_f32 = cfg.kv_dtype == LE_F32 && wide_tiles <= kSmallF32;
@@ -262,16 +262,16 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   // the chain of a tile's steps, the others by their keys' bytes; a CU holds
   // two workgroups. So the wide ones are cut to one a CU, beside which the
   // narrow ones stream (256 rows behind 16384 keys, 32/8 heads x 128, and 64 to
-  // 1024 keys of their own: 176 us, with two a CU 208), or to two where the
-  // narrow ones are few (122 rows after 131072 keys: 340 us, with one a CU 436).
+  // 1024 keys of their own: 174 us, with two a CU 208), or to two where the
+  // narrow ones are few (122 rows after 131072 keys: 327 us, with one a CU 431).
   // The narrow ones are cut to the places left (64 rows behind 4096 keys and 16
-  // to 512 of their own, 14/2 heads x 64: 12.9 us, to 64 keys each 15.7), with
+  // to 512 of their own, 14/2 heads x 64: 12.9 us, uncut 14.8), with
   // an fp32 cache, whose products count here too, to one a CU (24 rows behind
-  // 1500 keys 12.0 us, in parts twice as long 15.2), but not where they fill the
+  // 1500 keys 11.3 us, in parts twice as long 14.0), but not where they fill the
   // chip as they are, up to 1024 keys (48 sequences of 5 to 700 keys, 8 kv
-  // heads: 19.6 us, cut at 512 keys 22.3).
+  // heads: 18.9 us, cut at 512 keys 22.8).
   // Wide fp32 tiles of head_dim 64, two a CU, hide each other's softmax (3 x 220
-  // rows behind 5200 keys, 12 heads: 131 us, one a CU 150), from 256 keys on (30
+  // rows behind 5200 keys, 12 heads: 129 us, one a CU 145), from 256 keys on (30
   // rows behind 8192, 32/4 heads: 32 us, cut at 128 keys 37); of head_dim 128
   // one fits.
   const int quantum = std::max(le::kPrefixTileKeys, bs);
@@ -279,7 +279,7 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   auto wide = [&](const Tile& t) { return static_cast<int>(t.rows.size()) * G > le::kPrefixNarrow; };
   // Narrow tiles of shared keys (kind 2) are few and long beside the sequences'
   // own ones, and cut apart from them (4 x 10 sequences of up to 4 rows behind
-  // 1184 keys and 3 of their own, 12 heads x 64: 13 us, together 24).
+  // 1184 keys and 3 of their own, 12 heads x 64: 12 us, together 24).
   auto kind = [&](const Tile& t) { return wide(t) ? 1 : t.causal ? 0 : 2; };
   std::vector<int64_t> len[3];
   int64_t work[3] = {0, 0, 0};
@@ -355,7 +355,7 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   // Where there are more workgroups than places, an item of a few keys is given
   // to one wave: alone it would keep four waves for the time of a few trips to
   // memory (256 rows behind 512 keys and 1 to 30 of their own, 32/8 heads x 128:
-  // 24 us, 33 without; 234 rows behind 80 and 3, fp32, 32/4 x 64: 16, 21; where
+  // 23 us, 33 without; 234 rows behind 80 and 3, fp32, 32/4 x 64: 15, 21; where
   // they all fit it is slower: 4 rows behind 512 keys and 8 to 100, 10.0 us
   // against 7.9; items up to 64 keys: 4 x 32 rows 13.2 us, 12.7).
   const bool full = n_items * cfg.kv_heads > places;
