@@ -350,7 +350,7 @@ size_t le_shared_prefix_workspace_size(const le_prefix_plan* plan);
  * block id outside [0, num_cache_blocks) reads as zeros. q, out and the caches
  * 16-byte aligned, a block of K less than 4 GiB (LE_EUNSUPPORTED otherwise). NaN
  * or inf in a V row reaches rows before it of the same slice that share its tile
- * of up to 128 columns. */
+ * of up to 128 columns. out must not overlap q (LE_EINVAL). */
 int le_shared_prefix_attention(const void* q, le_dtype act_dtype, const void* k_cache,
                                const void* v_cache, le_dtype kv_dtype, int64_t num_cache_blocks,
                                const le_prefix_plan* plan, float scale, void* out, void* workspace,

@@ -216,6 +216,10 @@ int le_shared_prefix_attention(const void* q, le_dtype act_dtype, const void* k_
   const size_t need = le_shared_prefix_workspace_size(plan);
   if (need > 0 && (!workspace || workspace_bytes < need)) return LE_ENOSPACE;
   if (need > 0 && !aligned16({workspace})) return LE_EUNSUPPORTED;
+  // a row of q is read by several workgroups, and at different times
+  const size_t rows = static_cast<size_t>(plan->n_tokens) * cfg.q_heads * cfg.head_dim * (act_dtype == LE_F32 ? 4 : 2);
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
+  if (q0 < o0 + rows && o0 < q0 + rows) return LE_EINVAL;
   const char* dev = static_cast<const char*>(plan->dev);
   auto arr = [&](int64_t off) { return reinterpret_cast<const int32_t*>(dev + off); };
   le::PrefixParams p{};

@@ -173,6 +173,7 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   for (int i = 0; i < n_slices; i++) {
     const le_step_slice& s = slices[i];
     if (s.len <= 0 || s.start < 0 || s.num_blocks < 0 || s.len > INT32_MAX - s.start) return LE_EINVAL;
+    if (s.start + s.len > INT32_MAX - 4096) return LE_EUNSUPPORTED;  // a kernel counts on to the end of a tile
     if (s.num_blocks > 0 && !s.blocks) return LE_EINVAL;
     table[i] = &slices[seen.emplace(s.seq_key, i).first->second];
     if ((s.start + s.len - 1) / bs >= table[i]->num_blocks) return LE_EINVAL;  // a position without a block

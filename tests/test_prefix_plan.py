@@ -235,6 +235,22 @@ def test_blocks_past_32_bit_offsets_are_refused():
     assert st == _lib.LE_EUNSUPPORTED
 
 
+def test_overlapping_outputs_and_endless_sequences_are_refused():
+    plan = pack([(np.arange(30), 400, 1), (np.arange(30), 410, 1)])
+    P, L = plan.plan, _lib.load()
+    P.dev = 4096
+    rows = 2 * 14 * 64 * 2
+    for out in (1 << 20, (1 << 20) + rows - 16, (1 << 20) - rows + 16):
+        st = L.le_shared_prefix_attention(1 << 20, 1, 4096, 4096, 1, 64, ctypes.byref(P), 1.0, out, 1 << 24, 1 << 30, None)
+        assert st == _lib.LE_EINVAL
+    one = (_lib.StepSlice * 1)()
+    block = np.zeros(1 << 22, dtype=np.int32)
+    for start, want in ((2**31 - 2, _lib.LE_EUNSUPPORTED), (2**31 - 4096, _lib.LE_EUNSUPPORTED), (2**31 - 1, _lib.LE_EINVAL)):
+        one[0] = _lib.StepSlice(0, start, 1, 1, block.size, block.ctypes.data, None)
+        cfg = _lib.PlanConfig(14, 2, 64, 512, _lib.LE_BF16, 0, 0, 0, 0, 0)
+        assert L.le_prefix_plan_step(one, 1, ctypes.byref(cfg), None, 0, ctypes.byref(_lib.PrefixStepPlan())) == want
+
+
 def test_verify_refusals_without_launch():
     L = _lib.load()
     fake, odd, nul = ctypes.c_void_p(4096), ctypes.c_void_p(4104), ctypes.c_void_p(0)
