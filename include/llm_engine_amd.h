@@ -346,7 +346,8 @@ size_t le_shared_prefix_workspace_size(const le_prefix_plan* plan);
 /* out[t] for every row of the plan, as le_ragged_paged_attention on the same
  * slices. The step's own K/V rows are in the cache already. With q and the
  * cache of one 16-bit type the products are that type's (the softmax weights
- * rounded to it, once or in two terms); with any other pair they are fp32. A
+ * rounded to it, once or in two terms); with any other pair they have fp32
+ * accuracy (fp32 q over a bf16 cache: in three bf16 terms, faster). A
  * block id outside [0, num_cache_blocks) reads as zeros. q, out and the caches
  * 16-byte aligned, a block of K less than 4 GiB (LE_EUNSUPPORTED otherwise). NaN
  * or inf in a V row reaches rows before it of the same slice that share its tile

@@ -1,4 +1,5 @@
-// Shared-prefix attention on the fp32 MFMA: fp32 activations or an fp32 cache.
+// Shared-prefix attention of fp32 accuracy: fp32 activations or an fp32 cache, or
+// two 16-bit types.
 #include "attention_prefix_wg.h"
 
 namespace le {
@@ -8,7 +9,7 @@ hipError_t attention_prefix_f32(const PrefixParams& p, int act_dtype, int kv_dty
     return with_dtype(kv_dtype, [&](auto kv) {
       using ACT = decltype(act);
       using KV = decltype(kv);
-      if constexpr (std::is_same_v<pfx::operand<ACT, KV>, float>) {
+      if constexpr (!std::is_same_v<ACT, KV> || sizeof(KV) == 4) {
         return p.head_dim == 64 ? pfx::launch_prefix<ACT, KV, 64>(p, stream)
                                 : pfx::launch_prefix<ACT, KV, 128>(p, stream);
       } else {

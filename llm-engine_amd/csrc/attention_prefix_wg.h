@@ -29,8 +29,11 @@
 // Arithmetic: q, K and V of one 16-bit type use that type's MFMA, and the
 // softmax weights are rounded to it (the row sum is of the rounded weights; in
 // the key-sharing case, which has the matrix cores to spare, they are two
-// 16-bit terms instead). Anything else (fp32 activations or an fp32 cache)
-// uses the fp32 MFMA on widened operands.
+// 16-bit terms instead). fp32 q over a bf16 cache, and their weights, are three
+// bf16 terms each: products of 24 bits, in a fifth of the fp32 MFMA's cycles (256
+// rows behind 16384 keys and 64 to 1024 of their own, 32/8 heads x 128: 318 us, on
+// the fp32 MFMA 868).
+// Anything else uses the fp32 MFMA on widened operands.
 //
 // What bounds it: narrow tiles, HBM (256 sequences of 64 to 1024 keys, 8 kv
 // heads x 128, bf16: 108 us, 5.4 TB/s of K and V); wide ones, the products and
@@ -59,9 +62,14 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef short bf16raw4 __attribute__((ext_vector_type(4)));
 
-// The operand type: the 16-bit type of both, or float.
+// The operand type: the 16-bit type of both, bf16 also under fp32 activations, or
+// float.
 template <typename ACT, typename KV>
-using operand = std::conditional_t<std::is_same_v<ACT, KV> && sizeof(KV) == 2, KV, float>;
+using operand = std::conditional_t<(std::is_same_v<ACT, KV> && sizeof(KV) == 2) ||
+                                       (std::is_same_v<ACT, float> && std::is_same_v<KV, bf16_t>), KV, float>;
+// Terms of the operand type that a q element is given in; softmax weights have
+// as many (one: rounded; 16 keys a wave: two).
+template <typename ACT, typename KV> constexpr int kTerms = !std::is_same_v<ACT, KV> && sizeof(operand<ACT, KV>) == 2 ? 3 : 1;
 
 // Products over 16 (wide: 32x32 tiles) or 32 (narrow: 16x16 tiles) dims, a
 // lane holding eight consecutive ones of its row of A and column of B; and
@@ -216,26 +224,46 @@ __device__ __forceinline__ Column column_of(const PrefixParams& p, const PrefixI
   return o;
 }
 
+// x as N terms of type S, the largest first. What they leave is 2^-25 of x with
+// three bf16 ones (an infinity is in the first alone).
+template <int N, typename S> __device__ __forceinline__ void split(float x, S (&t)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; k++) {
+    t[k] = static_cast<S>(x);
+    const float y = static_cast<float>(t[k]);
+    if (k + 1 < N) x = y - y == 0.f ? x - y : 0.f;
+  }
+}
+// the same of a weight, which is at most some hundreds
+template <int N, typename S> __device__ __forceinline__ void split_weight(float x, S (&t)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; k++) {
+    t[k] = static_cast<S>(x);
+    if (k + 1 < N) x -= static_cast<float>(t[k]);
+  }
+}
+
 // eight elements of a column's q from dim d on, with the scale's sign
-template <typename ACT, typename X>
-__device__ __forceinline__ typename mm<X>::frag q_frag(const PrefixParams& p, const Column& c, int hd, int d) {
+template <typename ACT, typename X, int TERMS>
+__device__ __forceinline__ void q_frag(const PrefixParams& p, const Column& c, int hd, int d, typename mm<X>::frag (&r)[TERMS]) {
   const ACT* q = static_cast<const ACT*>(p.q) + (static_cast<int64_t>(c.token) * p.q_heads + c.head) * hd + d;
-  if constexpr (sizeof(X) == 2) {  // the same type: bits
+  if constexpr (sizeof(X) == 2 && TERMS == 1) {  // the same type: bits
     u32x4 raw = *reinterpret_cast<const u32x4*>(q);
     const uint32_t sign = p.negate ? 0x80008000u : 0u, keep = c.ok ? ~0u : 0u;
 #pragma unroll
     for (int e = 0; e < 4; e++) raw[e] = (raw[e] ^ sign) & keep;
-    return __builtin_bit_cast(typename mm<X>::frag, raw);
-  }
-  float f[8];
-  elem<ACT>::load8(q, f);
-  typename mm<X>::frag r;
+    r[0] = __builtin_bit_cast(typename mm<X>::frag, raw);
+  } else {
+    float f[8];
+    elem<ACT>::load8(q, f);
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const float x = c.ok ? (p.negate ? -f[e] : f[e]) : 0.f;
-    r[e] = static_cast<typename mm<X>::scalar>(x);
+    for (int e = 0; e < 8; e++) {
+      typename mm<X>::scalar t[TERMS];
+      split(c.ok ? (p.negate ? -f[e] : f[e]) : 0.f, t);
+#pragma unroll
+      for (int k = 0; k < TERMS; k++) r[k][e] = t[k];
+    }
   }
-  return r;
 }
 
 // Where a row's part is written: its record's accumulator and (m, l).
@@ -387,9 +415,10 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
   typename Loader<KV, HD>::Stage first;
   ld.issue(first, 0);
   const Column c = column_of(p, it, row, kvh, wave * 32 + col);
-  typename M::frag qb[KS];
+  constexpr int TERMS = kTerms<ACT, KV>;
+  typename M::frag qb[KS][TERMS];
 #pragma unroll
-  for (int ks = 0; ks < KS; ks++) qb[ks] = q_frag<ACT, X>(p, c, HD, ks * 16 + half * 8);
+  for (int ks = 0; ks < KS; ks++) q_frag<ACT, X>(p, c, HD, ks * 16 + half * 8, qb[ks]);
   // the wave's keys: none past the last one that any of its columns sees, and
   // no mask up to the first that one does not (columns without a row aside)
   const bool any = row_index(p, wave * 32) < it.n_rows;
@@ -435,7 +464,8 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
     if constexpr (sizeof(X) == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      s[i % U] = M::wide(kf[i % kAhead], qb[i / U], s[i % U]);
+#pragma unroll
+      for (int k = 0; k < TERMS; k++) s[i % U] = M::wide(kf[i % kAhead], qb[i / U][k], s[i % U]);
       if (i + kAhead < N) kf[i % kAhead] = k_frag(i + kAhead);
       if constexpr (sizeof(X) == 2) __builtin_amdgcn_sched_barrier(0);
     }
@@ -489,16 +519,22 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
       }
     } else {
       // weights g: those of accumulators 8 (g % 2) .. + 7 of s[g / 2]
-      typename M::frag pb[2 * U];
+      typename M::frag pb[2 * U][TERMS];
       auto weights = [&](int g, int e) {
         const f32x16& x = s[g / 2];
         const int at = 8 * (g % 2) + e;
-        typename M::pair w;
-        w[0] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[at], scale, -base)));
-        w[1] = static_cast<typename M::scalar>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[at + 1], scale, -base)));
-        pb[g][e] = w[0];
-        pb[g][e + 1] = w[1];
-        lsum = M::sum2(w, lsum);
+        const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[at], scale, -base));
+        const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[at + 1], scale, -base));
+        typename M::scalar t0[TERMS], t1[TERMS];
+        split_weight(w0, t0);
+        split_weight(w1, t1);
+#pragma unroll
+        for (int k = 0; k < TERMS; k++) {
+          pb[g][k][e] = t0[k];
+          pb[g][k][e + 1] = t1[k];
+        }
+        if constexpr (TERMS == 1) lsum = M::sum2(typename M::pair{t0[0], t1[0]}, lsum);
+        else lsum += w0 + w1;
       };
       // Beside each product: the read of the fragment two products on, and its
       // share of the next 16 keys' weights.
@@ -522,7 +558,8 @@ __device__ __forceinline__ void wide_item(const PrefixParams& p, const PrefixIte
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         const int g = i / DT, d = i % DT;
-        acc[d] = M::wide(vf[i % kAheadV], pb[g], acc[d]);
+#pragma unroll
+        for (int k = 0; k < TERMS; k++) acc[d] = M::wide(vf[i % kAheadV], pb[g][k], acc[d]);
         if (i + kAheadV < NV) vf[i % kAheadV] = v_frag(i + kAheadV);
         if (g + 1 < 2 * U) {
 #pragma unroll
@@ -580,12 +617,13 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
   typename Loader<KV, HD, SOLO>::Stage first;
   ld.issue(first, 0);
   Column c[NC];
-  typename M::frag qb[NC][KS];
+  constexpr int TERMS = kTerms<ACT, KV>;
+  typename M::frag qb[NC][KS][TERMS];
 #pragma unroll
   for (int n = 0; n < NC; n++) {
     c[n] = column_of(p, it, rows[n], kvh, n * 16 + l16);
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) qb[n][ks] = q_frag<ACT, X>(p, c[n], HD, ks * 32 + g * 8);
+    for (int ks = 0; ks < KS; ks++) q_frag<ACT, X>(p, c[n], HD, ks * 32 + g * 8, qb[n][ks]);
   }
   if (!SOLO && wave == 0 && g == 0) {
 #pragma unroll
@@ -616,7 +654,9 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
     for (int ks = 0; ks < KS; ks++) {
       const auto ka = lds_frag<X, KV, HD>(b + l16 * L::ROW, fk, (ks * 32 + g * 8) * L::ES / 16);
 #pragma unroll
-      for (int n = 0; n < NC; n++) s[n] = M::narrow(ka, qb[n][ks], s[n]);
+      for (int n = 0; n < NC; n++)
+#pragma unroll
+        for (int k = 0; k < TERMS; k++) s[n] = M::narrow(ka, qb[n][ks][k], s[n]);
     }
     // accumulator i of a lane is key 4 g + i
     float w[NC][4];
@@ -655,13 +695,16 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
         }
       }
     } else {
-      typename mma16<KV>::v4 hi[NC], lo[NC];
+      constexpr int WT = TERMS == 1 ? 2 : TERMS;
+      typename mma16<KV>::v4 wt[NC][WT];
 #pragma unroll
       for (int n = 0; n < NC; n++) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          hi[n][i] = static_cast<typename M::scalar>(w[n][i]);
-          lo[n][i] = static_cast<typename M::scalar>(w[n][i] - static_cast<float>(hi[n][i]));
+          typename M::scalar t[WT];
+          split_weight(w[n][i], t);
+#pragma unroll
+          for (int k = 0; k < WT; k++) wt[n][k][i] = t[k];
         }
       }
       const int row = 4 * g + (l16 >> 2), piece = (l16 & 3) >> 1, f = L::f(row);
@@ -671,8 +714,8 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
         const auto va = lds_read_tr16<KV>(vp + (((d * 2 + piece) ^ f) << 4));
 #pragma unroll
         for (int n = 0; n < NC; n++) {
-          acc[n][d] = M::keys16(va, hi[n], acc[n][d]);
-          acc[n][d] = M::keys16(va, lo[n], acc[n][d]);
+#pragma unroll
+          for (int k = 0; k < WT; k++) acc[n][d] = M::keys16(va, wt[n][k], acc[n][d]);
         }
       }
     }
@@ -750,7 +793,7 @@ __device__ __forceinline__ void narrow_item(const PrefixParams& p, const PrefixI
 }
 
 template <typename ACT, typename KV, int HD>
-__global__ __launch_bounds__(kThreads, (std::is_same_v<operand<ACT, KV>, float> && HD > 64 ? 1 : 2)) void prefix_kernel(PrefixParams p) {
+__global__ __launch_bounds__(kThreads, (HD > 64 && (std::is_same_v<operand<ACT, KV>, float> || kTerms<ACT, KV> > 1) ? 1 : 2)) void prefix_kernel(PrefixParams p) {
   __shared__ Smem<KV, HD> sm;
   // an item's kv heads lie side by side: their rows are neighbours in the cache
   const uint32_t shared = static_cast<uint32_t>(p.n_items - p.n_solo) * p.kv_heads;
