@@ -31,7 +31,7 @@ constexpr int kMaxParts = 128;        // partitions of a tile
 constexpr int kCus = 256;             // MI355X
 constexpr int kWideCost = 2;          // time of a wide tile's keys, in narrow ones
 constexpr int kShortOwn = 256;        // keys of a sequence that few columns attend in narrow tiles
-constexpr int kSoloKeys = 32;         // keys of a narrow item up to which a wave takes it alone
+constexpr int kSoloKeys = 32;         // keys of a narrow item up to which a wave takes it alone (twice: in a very full step)
 constexpr int kExtra = 6;             // time of a 16-bit workgroup around its tiles, in LDS tiles
 constexpr int kMinF32 = 4;            // LDS tiles of an fp32 item that is not narrow, at least
 constexpr int kSmallF32 = 256;        // LDS tiles of wide fp32 items up to which narrow ones take their place
@@ -358,9 +358,12 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   // memory (256 rows behind 512 keys and 1 to 30 of their own, 32/8 heads x 128:
   // 23 us, 33 without; 234 rows behind 80 and 3, fp32, 32/4 x 64: 15, 21; where
   // they all fit it is slower: 4 rows behind 512 keys and 8 to 100, 10.0 us
-  // against 7.9; items up to 64 keys: 4 x 32 rows 13.2 us, 12.7).
-  const bool full = n_items * cfg.kv_heads > places;
-  auto solo = [&](const Placed& a) { return full && !wide(*a.tile) && a.item.key_end - a.item.key_begin <= kSoloKeys; };
+  // against 7.9). From twice the places on items of up to 64 keys too (186 fp32
+  // rows of 35 keys, 10 heads x 128: 22 us, 43; at 1.25 times, 4 x 32 rows with
+  // up to 200, 13.2 us, 12.7).
+  const int64_t load = n_items * cfg.kv_heads / places;
+  const int solo_keys = load >= 2 ? 2 * kSoloKeys : n_items * cfg.kv_heads > places ? kSoloKeys : 0;
+  auto solo = [&](const Placed& a) { return !wide(*a.tile) && a.item.key_end - a.item.key_begin <= solo_keys; };
   const auto first_solo = std::stable_partition(items.begin(), items.end(), [&](const Placed& a) { return !solo(a); });
 
   // ---- layout and copy ----

@@ -239,6 +239,14 @@ def test_many_short_sequences(gpu, heads, n, act, kv):
     s.check()
 
 
+@pytest.mark.parametrize("act,kv", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32")])
+def test_very_many_short_sequences(gpu, act, kv):
+    """Twice the workgroups that the chip holds: items of up to 64 keys take a wave."""
+    s = Step([(0, 6, 1 + i % 80, 1) for i in range(170)], WIDE, act=act, kv=kv, seed=25)
+    assert s.plan.plan.n_solo > 100
+    s.check()
+
+
 @pytest.mark.parametrize("kv", ["bf16", "f16", "f32"])
 def test_dead_cache_rows_are_not_read(gpu, kv):
     """NaN in every cache row that no sequence has computed (the rest of the last
