@@ -353,8 +353,8 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   }
   auto cost = [&](const Placed& a) { return static_cast<int64_t>(a.item.key_end - a.item.key_begin) * (wide(*a.tile) ? kWideCost : 1); };
   std::stable_sort(items.begin(), items.end(), [&](const Placed& a, const Placed& b) { return cost(a) > cost(b); });
-  // Where there are more workgroups than places, an item of a few keys is given
-  // to one wave: alone it would keep four waves for the time of a few trips to
+  // Where there are more workgroups than places, a sequence's item of a few keys
+  // is given to one wave: alone it would keep four waves for the time of a few trips to
   // memory (256 rows behind 512 keys and 1 to 30 of their own, 32/8 heads x 128:
   // 23 us, 33 without; 234 rows behind 80 and 3, fp32, 32/4 x 64: 15, 21; where
   // they all fit it is slower: 4 rows behind 512 keys and 8 to 100, 10.0 us
@@ -363,7 +363,7 @@ int plan_step(const le_step_slice* slices, int n_slices, const le_plan_config* c
   // up to 200, 13.2 us, 12.7).
   const int64_t load = n_items * cfg.kv_heads / places;
   const int solo_keys = load >= 2 ? 2 * kSoloKeys : n_items * cfg.kv_heads > places ? kSoloKeys : 0;
-  auto solo = [&](const Placed& a) { return !wide(*a.tile) && a.item.key_end - a.item.key_begin <= solo_keys; };
+  auto solo = [&](const Placed& a) { return kind(*a.tile) == 0 && a.item.key_end - a.item.key_begin <= solo_keys; };
   const auto first_solo = std::stable_partition(items.begin(), items.end(), [&](const Placed& a) { return !solo(a); });
 
   // ---- layout and copy ----

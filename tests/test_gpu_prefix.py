@@ -247,6 +247,14 @@ def test_very_many_short_sequences(gpu, act, kv):
     s.check()
 
 
+@pytest.mark.parametrize("heads", [LLAMA, (3, 3, 128)])
+def test_nothing_but_short_sequences(gpu, heads):
+    """Every item takes a wave; the last workgroup's waves are not all needed."""
+    s = Step([(i, 0, 1 + i % 64, 1 + min(i % 64, i % 3)) for i in range(701)], heads, seed=26)
+    assert s.plan.plan.n_solo == s.plan.plan.n_items == 701 and s.plan.workspace_size() == 0
+    s.check()
+
+
 @pytest.mark.parametrize("kv", ["bf16", "f16", "f32"])
 def test_dead_cache_rows_are_not_read(gpu, kv):
     """NaN in every cache row that no sequence has computed (the rest of the last
