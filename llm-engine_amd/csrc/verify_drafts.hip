@@ -11,7 +11,7 @@
 // mass max(e / S - q, 0), fp32 too; the factors log2(e) / T and 1 / S are kept in
 // two terms each, since their rounding would shift every weight of a row alike.
 // Sums (past eight tokens) and everything compared with a random number are
-// fp64: a border of the running mass is then off by about 1e-8, where an fp32
+// fp64: a border of the running mass is then off by about 1e-9, where an fp32
 // sum over 10^5 tokens moves it by 1e-5. (fp64 masses, which the weights' own
 // roundings do not merit: 64 sequences x 151936 tokens 4 us slower.)
 //
@@ -396,7 +396,7 @@ __device__ __forceinline__ int decide(const VerifyParams& p, VerifySmem& sm, int
 // The token: the piece that the border falls into, the wave's share of it, the
 // place in that.
 template <typename T, typename Q, bool TINY>
-__device__ __forceinline__ void pick(const VerifyParams& p, VerifySmem& sm, int seq, int32_t* out) {
+__device__ __forceinline__ void pick(const VerifyParams& p, VerifySmem& sm, int seq, float t, int32_t* out) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
   const Choice c = sm.choice;
   if (wave == 0) {
@@ -413,7 +413,8 @@ __device__ __forceinline__ void pick(const VerifyParams& p, VerifySmem& sm, int 
       if (residual && c.q_row >= 0) return __hip_atomic_load(mass + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       if (residual && i == less) return rest;
       const PieceStat a = st[i];
-      return a.m > -INFINITY ? a.s * (static_cast<double>(weight(a.m, c.m, c.c_hi, c.c_lo)) * inv) : 0.0;
+      // (in fp64: an fp32 factor would move all of the piece's mass by up to 6e-8 of it)
+      return a.m > -INFINITY ? a.s * (weight_f64(a.m, c.m, t) * inv) : 0.0;
     };
     double w0 = 0.0, total = 0.0;  // w0: of this lane's first piece
 #pragma unroll 1
@@ -554,7 +555,7 @@ __global__ __launch_bounds__(kPickThreads, 8) void verify_kernel(VerifyParams p)
     __syncthreads();
     if (!sm.last) return;
   }
-  pick<T, Q, TINY>(p, sm, seq, out + acc);
+  pick<T, Q, TINY>(p, sm, seq, t, out + acc);
 }
 
 }  // namespace
